@@ -713,14 +713,8 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   for (int i = 0; i < splits; ++i) {
     EncWork& w = e->work[i];
     if (!w.st) {
-      // high-priority streams: the runtime spreads normal-priority streams over its hardware
-      // queues (GPU_MAX_HW_QUEUES, 4) by use count, and in a process that already holds other
-      // streams both sub-batches can land on one queue and run one after the other (r06h trace
-      // of bench.py: both on queue 4, 15.0 ms against 13.1); the high-priority queues are a
-      // separate pool that nothing else in the process draws from
-      int lo = 0, hi = 0;
-      HIPC(hipDeviceGetStreamPriorityRange(&lo, &hi));
-      HIPC(hipStreamCreateWithPriority(&w.st, hipStreamNonBlocking, hi));
+      // default priority: work on streams of different priorities has hung MI355X boards
+      HIPC(hipStreamCreateWithFlags(&w.st, hipStreamNonBlocking));
     }
     if (!w.done) HIPC(hipEventCreateWithFlags(&w.done, hipEventDisableTiming));
     HIPC(hipStreamWaitEvent(w.st, e->ev_in, 0));
