@@ -1,0 +1,411 @@
+// int8_kernels.h — kernels of the 8-bit integer operators (C ABI in include/hcrag.h, host side in
+// int8_ops.hip; the encoder's HCR_I8 mode calls them):
+//   rows_to_int8_kernel   [residual add + LayerNorm / RMS norm | activation] -> int8 rows + scales
+//   int8_to_rows_kernel   the values that int8 rows and scales stand for
+//   int8_linear_direct    y = x . w^T of int8 rows, few tokens
+#pragma once
+#include "device_common.h"
+#include "gelu.h"
+#include "hcrag.h"
+
+namespace hcr {
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
+
+// -------------------------------------------------------------------------------------
+// Rows -> int8.  Per row: v = f(x) (below), a = max |v|, scale = a / 127,
+// q = round_half_even(v * (127 / a)).
+//   I8_QUANT  v = x                        I8_GELU  v = gelu(x) (exact-erf form)
+//   I8_LAYER  h = x + r, v = (h - mean) rsqrt(var + eps) g + b
+//   I8_RMS    h = x + r, v = h rsqrt(mean(h^2) + eps) g + b       (b may be absent)
+// A row is read once: its elements stay in registers (NCH chunks of 8 per thread) through the
+// centred second moment (as layernorm4_kernel) and the maximum.  Everything between the loads
+// and the stores is fp32: v is computed from the unrounded h, and the int8 rounding is the only
+// one q carries; sum (h) and y (v) are rounded once to their own types.
+// The maximum is taken over the bit patterns of |v|: an infinity or a NaN is larger than every
+// finite value, and such a row gets scale NaN and q = 0, so that a product with it is NaN.  A row
+// below 2^-100 counts as zeros (scale 0, q 0): 127 / a would leave fp32's range.
+// -------------------------------------------------------------------------------------
+enum : int { I8_QUANT = 0, I8_GELU = 1, I8_LAYER = 2, I8_RMS = 3 };
+
+struct I8RowArgs {
+  const void* x; int64_t ldx;
+  const void* r; int64_t ldr;      // residual (NULL: none)
+  void* sum; int64_t ldsum;        // h in r's type (NULL: not stored); may be r itself
+  void* y; int64_t ldy;            // v in yt (NULL: not stored); may be x or r itself
+  const float* g; const float* b;  // (b NULL: 0)
+  int8_t* q; int64_t ldq;
+  float* scale;
+  int64_t rows;
+  int cols;
+  float eps;
+  int xt, rt, yt;                  // hcr_dtype of x, r (and sum), y
+  int vec;                         // every row of x, r, sum, y, g, b starts on 16 bytes
+};
+
+struct I8Raw { uint4 a, b; };      // 8 elements as loaded: 16-bit types in a, f32 in a and b
+
+// elements [i, i + 8) of a row, n of them in the row (n >= 8: whole chunk)
+__device__ __forceinline__ void i8_load(I8Raw& o, const char* row, bool f32, int i, int n, bool vec) {
+  if (vec && n >= 8) {
+    if (f32) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + (size_t)i * 4);
+      o.a = p[0];
+      o.b = p[1];
+    } else {
+      o.a = *reinterpret_cast<const uint4*>(row + (size_t)i * 2);
+    }
+    return;
+  }
+  uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+  if (f32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) if (e < n) w[e] = reinterpret_cast<const uint32_t*>(row)[i + e];
+    o.b = uint4{w[4], w[5], w[6], w[7]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) w[e >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(row)[i + e] << (16 * (e & 1));
+  }
+  o.a = uint4{w[0], w[1], w[2], w[3]};
+}
+__device__ __forceinline__ void i8_convert(float (&v)[8], const I8Raw& o, int type) {
+  const uint32_t w[8] = {o.a.x, o.a.y, o.a.z, o.a.w, o.b.x, o.b.y, o.b.z, o.b.w};
+  if (type == HCR_F32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+  } else if (type == HCR_BF16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float((e & 1) ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+      v[e] = (float)__builtin_bit_cast(_Float16, h);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t i8_bits16(float v) { return __builtin_bit_cast(uint16_t, (T)v); }
+__device__ __forceinline__ void i8_store(char* row, int type, int i, int n, bool vec, const float (&v)[8]) {
+  if (type == HCR_F32) {
+    float* p = reinterpret_cast<float*>(row) + i;
+    if (vec && n >= 8) {
+      reinterpret_cast<float4*>(p)[0] = float4{v[0], v[1], v[2], v[3]};
+      reinterpret_cast<float4*>(p)[1] = float4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) if (e < n) p[e] = v[e];
+    }
+    return;
+  }
+  uint32_t h[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = type == HCR_BF16 ? i8_bits16<__bf16>(v[e]) : i8_bits16<_Float16>(v[e]);
+  uint16_t* p = reinterpret_cast<uint16_t*>(row) + i;
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint4*>(p) = uint4{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) if (e < n) p[e] = (uint16_t)h[e];
+  }
+}
+
+// sum / maximum over the WAVES waves that share a row (WAVES == 1: each wave has its own row)
+template <int WAVES>
+__device__ __forceinline__ float i8_row_sum(float s, float* red, int wave, int lane) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+  if constexpr (WAVES > 1) {
+    __syncthreads();               // (the previous reduction's reads of red are done)
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += red[w];
+  }
+  return s;
+}
+template <int WAVES>
+__device__ __forceinline__ uint32_t i8_row_max(uint32_t s, float* red, int wave, int lane) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) s = max(s, (uint32_t)__shfl_xor((int)s, m, 64));
+  if constexpr (WAVES > 1) {
+    __syncthreads();
+    if (lane == 0) red[wave] = __uint_as_float(s);
+    __syncthreads();
+    s = 0u;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s = max(s, __float_as_uint(red[w]));
+  }
+  return s;
+}
+
+// One row per WAVES waves; WAVES == 1 puts 4 rows in a workgroup.  Covers cols <= 512 WAVES NCH.
+template <int MODE, int WAVES, int NCH>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
+rows_to_int8_kernel(I8RowArgs a) {
+  __shared__ float red[WAVES > 1 ? WAVES : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  if (WAVES == 1 && row >= a.rows) return;
+  const int tid = WAVES == 1 ? lane : threadIdx.x;
+  constexpr int NTH = 64 * WAVES;
+  constexpr bool NORM = MODE == I8_LAYER || MODE == I8_RMS;
+  const bool vec = a.vec != 0;
+  const bool x32 = a.xt == HCR_F32, r32 = a.rt == HCR_F32;
+  const char* xr = reinterpret_cast<const char*>(a.x) + row * a.ldx * (x32 ? 4 : 2);
+  const char* rr = reinterpret_cast<const char*>(a.r) + row * a.ldr * (r32 ? 4 : 2);
+  I8Raw xs[NCH], rs[NORM ? NCH : 1];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int i = (tid + NTH * c) * 8;
+    xs[c] = I8Raw{};
+    if (i < a.cols) i8_load(xs[c], xr, x32, i, a.cols - i, vec);
+  }
+  if constexpr (NORM) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int i = (tid + NTH * c) * 8;
+      rs[c] = I8Raw{};
+      if (a.r && i < a.cols) i8_load(rs[c], rr, r32, i, a.cols - i, vec);
+    }
+  }
+  float v[NCH][8];                 // (elements past the row's end are 0)
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    i8_convert(v[c], xs[c], a.xt);
+    if constexpr (NORM) {
+      if (a.r) {
+        float r[8];
+        i8_convert(r, rs[c], a.rt);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[c][e] += r[e];
+      }
+    }
+    if constexpr (MODE == I8_GELU) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = gelu_erf(v[c][e]);
+    }
+  }
+  bool overflow = false;
+  if constexpr (NORM) {
+    float mean = 0.f;
+    if constexpr (MODE == I8_LAYER) {
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c)
+        s += ((v[c][0] + v[c][1]) + (v[c][2] + v[c][3])) + ((v[c][4] + v[c][5]) + (v[c][6] + v[c][7]));
+      mean = i8_row_sum<WAVES>(s, red, wave, lane) / (float)a.cols;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int n = a.cols - (tid + NTH * c) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = e < n ? v[c][e] - mean : 0.f;
+        s = fmaf(d, d, s);
+      }
+    }
+    const float var = i8_row_sum<WAVES>(s, red, wave, lane) / (float)a.cols;
+    overflow = !(var < INFINITY);  // the squares left fp32's range: the row is not representable
+    const float rstd = rsqrtf(var + a.eps);
+    if (a.sum) {
+      char* sr = reinterpret_cast<char*>(a.sum) + row * a.ldsum * (r32 ? 4 : 2);
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int i = (tid + NTH * c) * 8;
+        if (i < a.cols) i8_store(sr, a.rt, i, a.cols - i, vec, v[c]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int i = (tid + NTH * c) * 8, n = a.cols - i;
+      if (n <= 0) continue;
+      I8Raw raw;
+      float g[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      i8_load(raw, reinterpret_cast<const char*>(a.g), true, i, n, vec);
+      i8_convert(g, raw, HCR_F32);
+      if (a.b) {
+        i8_load(raw, reinterpret_cast<const char*>(a.b), true, i, n, vec);
+        i8_convert(b, raw, HCR_F32);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = e < n ? fmaf((v[c][e] - mean) * rstd, g[e], b[e]) : 0.f;
+    }
+    if (a.y) {
+      char* yr = reinterpret_cast<char*>(a.y) + row * a.ldy * (a.yt == HCR_F32 ? 4 : 2);
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int i = (tid + NTH * c) * 8;
+        if (i < a.cols) i8_store(yr, a.yt, i, a.cols - i, vec, v[c]);
+      }
+    }
+  }
+  uint32_t m = overflow ? 0x7FC00000u : 0u;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[c][e]) & 0x7FFFFFFFu);
+  m = i8_row_max<WAVES>(m, red, wave, lane);
+  const float amax = __uint_as_float(m);
+  const bool bad = m >= 0x7F800000u;
+  const bool zero = bad || amax < 0x1p-100f;
+  const float inv = zero ? 0.f : 127.f / amax;
+  if (tid == 0) a.scale[row] = bad ? __uint_as_float(0x7FC00000u) : zero ? 0.f : amax / 127.f;
+  int8_t* qr = a.q + row * a.ldq;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int i = (tid + NTH * c) * 8, n = a.cols - i;
+    if (n <= 0) continue;
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // (|v inv| <= 127 (1 + 2^-23), which rounds to 127; bad and zero rows are 0 whatever v is)
+      const int qe = zero ? 0 : (int)rintf(v[c][e] * inv);
+      w[e >> 2] |= ((uint32_t)qe & 255u) << (8 * (e & 3));
+    }
+    if (n >= 8) *reinterpret_cast<uint2*>(qr + i) = uint2{w[0], w[1]};   // (q rows start on 16 bytes)
+    else
+      for (int e = 0; e < n; ++e) qr[i + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
+  }
+}
+
+// out = q * scale, rounded once to the output's type.  One thread per 8 elements.
+__global__ void __launch_bounds__(256)
+int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t rows,
+                    int cols, void* __restrict__ out, int ot, int64_t ldo, int vec) {
+  const int per = (cols + 7) >> 3;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / per;
+  if (row >= rows) return;
+  const int i = (int)(id - row * per) * 8, n = cols - i;
+  uint32_t w[2] = {0u, 0u};
+  const int8_t* qr = q + row * ldq + i;
+  if (n >= 8) {
+    const uint2 u = *reinterpret_cast<const uint2*>(qr);
+    w[0] = u.x; w[1] = u.y;
+  } else {
+    for (int e = 0; e < n; ++e) w[e >> 2] |= (uint32_t)(uint8_t)qr[e] << (8 * (e & 3));
+  }
+  const float s = scale[row];
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * s;
+  i8_store(reinterpret_cast<char*>(out) + row * ldo * (ot == HCR_F32 ? 4 : 2), ot, i, n, vec != 0, v);
+}
+
+// -------------------------------------------------------------------------------------
+// y[t][f] = (sum_k x[t][k] w[f][k]) * sx[t] * sw[f] + bias[f].  The sum is exact in int32
+// (|x w| <= 2^14, K <= 131071), so any split of k gives the same bits; the conversion to fp32
+// rounds it once (sums above 2^24), and y is rounded once more to its type.
+// K need not fill a stage: w's bytes at k >= K are replaced by zeros in registers, so what the
+// padding of either operand holds does not matter.
+// -------------------------------------------------------------------------------------
+struct I8LinearArgs {
+  const int8_t* x; int64_t ldx; const float* sx;
+  const int8_t* w; int64_t ldw; const float* sw;
+  const float* bias;               // (NULL: 0)
+  void* out; int64_t ldo; int ot;  // hcr_dtype of out
+  int T, N, K;
+  int vec;                         // out's rows start on 4 elements
+};
+
+__device__ __forceinline__ intx4 i8_mfma(intx4 a, intx4 b, intx4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+// bytes of a 16-byte chunk that starts n bytes before the row's end, the others zero (n >= 16: all)
+__device__ __forceinline__ intx4 i8_keep(intx4 v, int n) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int left = n - 4 * d;
+    v[d] = left >= 4 ? v[d] : left <= 0 ? 0 : v[d] & (int)((1u << (8 * left)) - 1u);
+  }
+  return v;
+}
+
+// 4 consecutive features of token t
+__device__ __forceinline__ void i8_store_out4(const I8LinearArgs& a, int64_t t, int f, const float (&v)[4]) {
+  if (a.ot == HCR_F32) {
+    float* p = reinterpret_cast<float*>(a.out) + t * a.ldo + f;
+    if (a.vec && f + 4 <= a.N) *reinterpret_cast<float4*>(p) = float4{v[0], v[1], v[2], v[3]};
+    else
+#pragma unroll
+      for (int r = 0; r < 4; ++r) if (f + r < a.N) p[r] = v[r];
+    return;
+  }
+  uint32_t h[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) h[r] = a.ot == HCR_BF16 ? i8_bits16<__bf16>(v[r]) : i8_bits16<_Float16>(v[r]);
+  uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + t * a.ldo + f;
+  if (a.vec && f + 4 <= a.N) *reinterpret_cast<uint2*>(p) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+  else
+#pragma unroll
+    for (int r = 0; r < 4; ++r) if (f + r < a.N) p[r] = (uint16_t)h[r];
+}
+
+// Operands straight from memory to the matrix cores: 16 features x 16 TB tokens per workgroup,
+// whose KW waves take every KW-th 128-byte piece of the rows (a lane's 32 bytes are contiguous,
+// a row's 128 bytes one line; the contraction order is the same for both operands) and add their
+// int32 sums through LDS.
+template <int TB, int KW>
+__global__ void __launch_bounds__(64 * KW)
+int8_linear_direct(I8LinearArgs a) {
+  __shared__ __attribute__((aligned(16))) intx4 red[KW][TB][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int li = lane & 15, lg = lane >> 4;
+  const unsigned nfb = (unsigned)((a.N + 15) >> 4);
+  const int f0 = (int)(blockIdx.x % nfb) * 16, t0 = (int)(blockIdx.x / nfb) * (16 * TB);
+  const int8_t* wr = a.w + (int64_t)min(f0 + li, a.N - 1) * a.ldw;
+  const int8_t* xr[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) xr[b] = a.x + (int64_t)min(t0 + 16 * b + li, a.T - 1) * a.ldx;
+  intx4 acc[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) acc[b] = intx4{0, 0, 0, 0};
+  const int whole = a.K / 128 * 128;
+  for (int k = wave * 128; k < whole; k += KW * 128) {
+    const intx4* wp = reinterpret_cast<const intx4*>(wr + k + lg * 32);
+    const intx4 w0 = wp[0], w1 = wp[1];
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      const intx4* xp = reinterpret_cast<const intx4*>(xr[b] + k + lg * 32);
+      acc[b] = i8_mfma(w0, xp[0], acc[b]);
+      acc[b] = i8_mfma(w1, xp[1], acc[b]);
+    }
+  }
+  if (whole < a.K && (whole / 128) % KW == wave) {      // the rows' last, partial piece
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = whole + lg * 32 + j * 16, n = a.K - k;
+      const int kk = n > 0 ? k : 0;                     // (a chunk past the row: any, times 0)
+      const intx4 w0 = i8_keep(*reinterpret_cast<const intx4*>(wr + kk), n);
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+        acc[b] = i8_mfma(w0, *reinterpret_cast<const intx4*>(xr[b] + kk), acc[b]);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < TB; ++b) red[wave][b][lane] = acc[b];
+  __syncthreads();
+  for (int b = wave; b < TB; b += KW) {
+    intx4 s = red[0][b][lane];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) s += red[w][b][lane];
+    // lane: features f0 + 4 lg .. + 3 of token t0 + 16 b + li
+    const int t = t0 + 16 * b + li, f = f0 + 4 * lg;
+    if (t >= a.T || f >= a.N) continue;
+    const float sx = a.sx[t];
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int fr = min(f + r, a.N - 1);
+      v[r] = fmaf((float)s[r] * sx, a.sw[fr], a.bias ? a.bias[fr] : 0.f);
+    }
+    i8_store_out4(a, t, f, v);
+  }
+}
+
+}  // namespace hcr

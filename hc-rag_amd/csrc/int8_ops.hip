@@ -1,0 +1,157 @@
+// int8_ops.hip — host side of the 8-bit integer operators' C ABI (include/hcrag.h): argument
+// checks and the choice of a kernel.  Nothing here allocates, synchronises or keeps state, so
+// every call can be captured into a graph and run from several threads and streams at once.
+#include <hip/hip_runtime.h>
+
+#include "int8_kernels.h"
+#include "int8_ops.h"
+#include "host_common.h"
+
+using namespace hcr;
+
+namespace hcr {
+
+template <int MODE, int WAVES, int NCH>
+static void launch_rows(const I8RowArgs& a, hipStream_t st) {
+  const unsigned grid = WAVES == 1 ? (unsigned)((a.rows + 3) / 4) : (unsigned)a.rows;
+  hipLaunchKernelGGL((rows_to_int8_kernel<MODE, WAVES, NCH>), dim3(grid), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0,
+                     st, a);
+}
+template <int MODE>
+static void launch_rows_mode(const I8RowArgs& a, hipStream_t st) {
+  if (a.cols <= 512) launch_rows<MODE, 1, 1>(a, st);
+  else if (a.cols <= 1024) launch_rows<MODE, 1, 2>(a, st);
+  else if (a.cols <= 2048) launch_rows<MODE, 1, 4>(a, st);
+  else if (a.cols <= 4096) launch_rows<MODE, 4, 2>(a, st);
+  else if (a.cols <= 8192) launch_rows<MODE, 4, 4>(a, st);
+  else launch_rows<MODE, 16, 4>(a, st);
+}
+
+int int8_rows_launch(int mode, const I8RowArgs& a, hipStream_t st) {
+  if (mode == I8_QUANT) launch_rows_mode<I8_QUANT>(a, st);
+  else if (mode == I8_GELU) launch_rows_mode<I8_GELU>(a, st);
+  else if (mode == I8_LAYER) launch_rows_mode<I8_LAYER>(a, st);
+  else launch_rows_mode<I8_RMS>(a, st);
+  HIPC(hipGetLastError());
+  return HCR_OK;
+}
+
+int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
+  const int64_t blocks = (int64_t)((a.N + 15) / 16) * ((a.T + 63) / 64);
+  if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many outputs for one call");
+  hipLaunchKernelGGL((int8_linear_direct<4, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  HIPC(hipGetLastError());
+  return HCR_OK;
+}
+
+}  // namespace hcr
+
+static size_t float_size(int dt) { return dt == HCR_F32 ? 4 : 2; }
+static bool is_float(int dt) { return dt == HCR_F16 || dt == HCR_BF16 || dt == HCR_F32; }
+static bool on(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// a [rows][cols] operand of a floating type: its type, stride and alignment
+static int check_floats(const char* what, const void* p, int dt, int64_t ld, int cols) {
+  if (!is_float(dt)) return hcr_set_errorf(HCR_EINVAL, "%s: dtype must be HCR_F16, HCR_BF16 or HCR_F32, got %d", what, dt);
+  if (ld < cols) return hcr_set_errorf(HCR_EINVAL, "%s: row stride %lld is below %d columns", what, (long long)ld, cols);
+  if (!on(p, float_size(dt))) return hcr_set_errorf(HCR_EINVAL, "%s: not aligned to its elements", what);
+  return HCR_OK;
+}
+static int check_int8(const char* what, const void* p, int64_t ld, int cols) {
+  if (ld < cols) return hcr_set_errorf(HCR_EINVAL, "%s: row stride %lld is below %d columns", what, (long long)ld, cols);
+  if (!on(p, 16) || (ld & 15))
+    return hcr_set_errorf(HCR_EINVAL, "%s: int8 rows must start on 16 bytes (aligned pointer, row stride a multiple of 16)", what);
+  return HCR_OK;
+}
+static int check_rows(int64_t rows, int cols, int64_t max_cols) {
+  if (rows < 0 || rows > kI8MaxRows) return hcr_set_errorf(HCR_EINVAL, "rows must be in [0, 2^30], got %lld", (long long)rows);
+  if (cols < 1 || cols > max_cols) return hcr_set_errorf(HCR_EINVAL, "cols must be in [1, %lld], got %d", (long long)max_cols, cols);
+  return HCR_OK;
+}
+// rows that start on 16 bytes, so that whole chunks of 8 elements are aligned vectors
+static bool rows_on16(const void* p, int dt, int64_t ld) { return on(p, 16) && ld * (int64_t)float_size(dt) % 16 == 0; }
+
+extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int cols, int act,
+                                     int8_t* d_q, int64_t ldq, float* d_scale, void* stream) {
+  CHECK(check_rows(rows, cols, kI8MaxRowCols));
+  if (act != HCR_ACT_NONE && act != HCR_ACT_GELU) return hcr_set_errorf(HCR_EINVAL, "unknown activation %d", act);
+  if (rows == 0) return HCR_OK;
+  if (!d_x || !d_q || !d_scale) return hcr_set_error(HCR_EINVAL, "NULL buffer");
+  CHECK(check_floats("x", d_x, x_dtype, ldx, cols));
+  CHECK(check_int8("q", d_q, ldq, cols));
+  if (!on(d_scale, 4)) return hcr_set_error(HCR_EINVAL, "scale: not aligned to its elements");
+  I8RowArgs a{};
+  a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
+  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = cols;
+  a.vec = rows_on16(d_x, x_dtype, ldx);
+  return int8_rows_launch(act == HCR_ACT_GELU ? I8_GELU : I8_QUANT, a, (hipStream_t)stream);
+}
+
+extern "C" int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, const void* d_residual,
+                                          int r_dtype, int64_t ldr, int64_t rows, int cols, int norm,
+                                          const float* d_weight, const float* d_bias, float eps, void* d_sum,
+                                          int64_t ldsum, void* d_norm, int norm_dtype, int64_t ldnorm, int8_t* d_q,
+                                          int64_t ldq, float* d_scale, void* stream) {
+  CHECK(check_rows(rows, cols, kI8MaxRowCols));
+  if (norm != HCR_NORM_LAYER && norm != HCR_NORM_RMS) return hcr_set_errorf(HCR_EINVAL, "unknown norm %d", norm);
+  if (!(eps >= 0.f)) return hcr_set_error(HCR_EINVAL, "eps must be >= 0");
+  if (d_sum && !d_residual) return hcr_set_error(HCR_EINVAL, "a sum output needs a residual");
+  if (rows == 0) return HCR_OK;
+  if (!d_x || !d_weight || !d_q || !d_scale) return hcr_set_error(HCR_EINVAL, "NULL buffer");
+  CHECK(check_floats("x", d_x, x_dtype, ldx, cols));
+  if (d_residual) CHECK(check_floats("residual", d_residual, r_dtype, ldr, cols));
+  if (d_sum) CHECK(check_floats("sum", d_sum, r_dtype, ldsum, cols));
+  if (d_norm) CHECK(check_floats("norm output", d_norm, norm_dtype, ldnorm, cols));
+  CHECK(check_int8("q", d_q, ldq, cols));
+  if (!on(d_scale, 4) || !on(d_weight, 4) || !on(d_bias, 4))
+    return hcr_set_error(HCR_EINVAL, "scale, weight or bias: not aligned to its elements");
+  I8RowArgs a{};
+  a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
+  a.r = d_residual; a.ldr = ldr; a.rt = d_residual ? r_dtype : HCR_F32;
+  a.sum = d_sum; a.ldsum = ldsum;
+  a.y = d_norm; a.ldy = ldnorm; a.yt = norm_dtype;
+  a.g = d_weight; a.b = d_bias; a.eps = eps;
+  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = cols;
+  a.vec = rows_on16(d_x, x_dtype, ldx) && on(d_weight, 16) && on(d_bias, 16) &&
+          (!d_residual || rows_on16(d_residual, r_dtype, ldr)) && (!d_sum || rows_on16(d_sum, r_dtype, ldsum)) &&
+          (!d_norm || rows_on16(d_norm, norm_dtype, ldnorm));
+  return int8_rows_launch(norm == HCR_NORM_LAYER ? I8_LAYER : I8_RMS, a, (hipStream_t)stream);
+}
+
+extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows, int cols,
+                                       void* d_out, int out_dtype, int64_t ldo, void* stream) {
+  CHECK(check_rows(rows, cols, kI8MaxDepth));
+  if (rows == 0) return HCR_OK;
+  if (!d_q || !d_scale || !d_out) return hcr_set_error(HCR_EINVAL, "NULL buffer");
+  CHECK(check_int8("q", d_q, ldq, cols));
+  CHECK(check_floats("out", d_out, out_dtype, ldo, cols));
+  if (!on(d_scale, 4)) return hcr_set_error(HCR_EINVAL, "scale: not aligned to its elements");
+  const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
+  if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many elements for one call");
+  hipLaunchKernelGGL(int8_to_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, ldq,
+                     d_scale, rows, cols, d_out, out_dtype, ldo, rows_on16(d_out, out_dtype, ldo) ? 1 : 0);
+  HIPC(hipGetLastError());
+  return HCR_OK;
+}
+
+extern "C" int hcr_int8_linear_device(const int8_t* d_x, int64_t ldx, const float* d_x_scale, int64_t rows,
+                                      const int8_t* d_w, int64_t ldw, const float* d_w_scale, int features, int depth,
+                                      const float* d_bias, void* d_out, int out_dtype, int64_t ldo, void* stream) {
+  CHECK(check_rows(rows, depth, kI8MaxDepth));
+  if (features < 0 || features > kI8MaxRows)
+    return hcr_set_errorf(HCR_EINVAL, "features must be in [0, 2^30], got %d", features);
+  if (rows == 0 || features == 0) return HCR_OK;
+  if (!d_x || !d_x_scale || !d_w || !d_w_scale || !d_out) return hcr_set_error(HCR_EINVAL, "NULL buffer");
+  CHECK(check_int8("x", d_x, ldx, depth));
+  CHECK(check_int8("w", d_w, ldw, depth));
+  CHECK(check_floats("out", d_out, out_dtype, ldo, features));
+  if (!on(d_x_scale, 4) || !on(d_w_scale, 4) || !on(d_bias, 4))
+    return hcr_set_error(HCR_EINVAL, "scales or bias: not aligned to their elements");
+  I8LinearArgs a{};
+  a.x = d_x; a.ldx = ldx; a.sx = d_x_scale;
+  a.w = d_w; a.ldw = ldw; a.sw = d_w_scale;
+  a.bias = d_bias; a.out = d_out; a.ldo = ldo; a.ot = out_dtype;
+  a.T = (int)rows; a.N = features; a.K = depth;
+  a.vec = ldo % 4 == 0 && on(d_out, 4 * float_size(out_dtype));
+  return int8_linear_launch(a, (hipStream_t)stream);
+}

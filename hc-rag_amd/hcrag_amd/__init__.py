@@ -15,10 +15,22 @@ from .ingest import BatchedEmbeddingGenerator, EmbeddingStore
 from . import relevance
 from . import graph_relevance
 
+# the int8 operators work on torch tensors: torch is imported when one of them is first asked for
+_INT8 = ("Int8Rows", "quantize_rows", "norm_quantize", "int8_linear")
+
+
+def __getattr__(name):
+    if name in _INT8 or name == "int8":
+        import importlib
+        module = importlib.import_module(".int8", __name__)
+        return module if name == "int8" else getattr(module, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 __version__ = "0.3.0"
 
 __all__ = ["VectorIndex", "MultiDeviceIndex", "merge_topk_device", "EmbeddingSearch", "batch_semantic_similarity",
            "WordPieceTokenizer", "BertEncoder", "SentenceEmbedder", "MI355XEmbedding", "config_from_hf",
            "MINILM_L6_V2", "device_count", "lib", "HcrError", "HCR_F16", "HCR_BF16", "HCR_F32",
            "HCR_SCORE_COSINE", "HCR_SCORE_UNIT", "BatchedEmbeddingGenerator", "EmbeddingStore",
-           "relevance", "graph_relevance"]
+           "relevance", "graph_relevance", *_INT8]

@@ -16,6 +16,8 @@ LIB_PATH = os.environ.get(
 HCR_OK, HCR_EINVAL, HCR_EHIP, HCR_ERCCL, HCR_ENOMEM, HCR_EIO, HCR_EINTERNAL = 0, -1, -2, -3, -4, -5, -6
 HCR_F16, HCR_BF16, HCR_F32 = 0, 1, 2
 HCR_SCORE_COSINE, HCR_SCORE_UNIT = 0, 1
+HCR_ACT_NONE, HCR_ACT_GELU = 0, 1
+HCR_NORM_LAYER, HCR_NORM_RMS = 0, 1
 
 
 class HcrError(RuntimeError):
@@ -99,6 +101,17 @@ _SIGS = {
     "hcr_encode": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "hcr_encode_device": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
                                   c_void_p]),
+    "hcr_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
+                                      c_int64, c_void_p, c_void_p]),
+    "hcr_norm_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
+                                           c_int64, c_int, c_int, c_void_p, c_void_p, c_float,
+                                           c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p,
+                                           c_int64, c_void_p, c_void_p]),
+    "hcr_dequant_rows_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                                        c_int, c_int64, c_void_p]),
+    "hcr_int8_linear_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                       c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int64,
+                                       c_void_p]),
     "hcr_relevance_combine": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int, c_int64,
                                       c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                       c_void_p, c_int, c_int, c_void_p, c_int, c_void_p,

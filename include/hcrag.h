@@ -39,6 +39,11 @@ typedef enum {
 
 typedef enum { HCR_F16 = 0, HCR_BF16 = 1, HCR_F32 = 2 } hcr_dtype;
 
+/* What hcr_quant_rows_device applies to a value before it is quantised (GELU: exact-erf form). */
+typedef enum { HCR_ACT_NONE = 0, HCR_ACT_GELU = 1 } hcr_activation;
+/* The norm of hcr_norm_quant_rows_device. */
+typedef enum { HCR_NORM_LAYER = 0, HCR_NORM_RMS = 1 } hcr_norm;
+
 typedef enum {
   HCR_SCORE_COSINE = 0,     /* raw cosine: experiments/main.py:841 */
   HCR_SCORE_UNIT = 1        /* (cos + 1) / 2: experiments/isRelevant.py:208 */
@@ -333,6 +338,57 @@ int hcr_encode(hcr_encoder* enc, const int32_t* ids, const int32_t* mask, int64_
  * `stream` waits for). */
 int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_mask, int64_t n,
                       int S, float* d_out, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * 8-bit integer operators of the encoder's layers, on device buffers.  They are what an encoder
+ * whose linear layers run on 8-bit integers is made of; the reference computes those layers in
+ * fp32 (experiments/embedding_generator.py:124).
+ *
+ * int8 rows: q [rows][cols] of int8 with one fp32 scale per row; element = q * scale.  q's rows
+ * start on 16 bytes (16-byte aligned pointer, row stride ldq a multiple of 16; for one row too);
+ * bytes of a row past its columns are neither read as values nor written.  Strides (ld*) are in
+ * elements and at least the row's columns; other buffers need only their elements' alignment
+ * (rows that start on 16 bytes are read and written in vectors).
+ *
+ * Asynchronous on `stream` (a hipStream_t of the current device; NULL = the legacy default
+ * stream).  Nothing is allocated, waited for or kept between calls: calls may run at once from
+ * several threads and be captured into graphs.  0 rows (and 0 features): nothing is done.
+ * At most 2^30 rows and features; quantised rows of 1 .. 32768 columns.
+ *
+ * Quantisation of a row v: a = max |v|, scale = a / 127, q = round_half_even(v * (127 / a)), in
+ * fp32.  a < 2^-100: the row counts as zeros (q 0, scale 0).  A row that holds a NaN or an
+ * infinity, or whose squares leave fp32's range in a norm, gets q 0 and scale NaN, so that what is
+ * computed from it is NaN.
+ * ------------------------------------------------------------------------------------- */
+
+/* v = activation(x): int8 rows of x [rows][cols] (x_dtype HCR_F16 / HCR_BF16 / HCR_F32).  Weights
+ * [features][depth] are laid out by the same call: a channel is a row. */
+int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int cols,
+                          int activation, int8_t* d_q, int64_t ldq, float* d_scale, void* stream);
+
+/* h = x + residual (residual NULL: h = x); v = norm(h) * weight + bias (bias NULL: 0), with
+ * norm(h) = (h - mean) / sqrt(var + eps) (HCR_NORM_LAYER) or h / sqrt(mean(h^2) + eps)
+ * (HCR_NORM_RMS), all in fp32; int8 rows of v.  d_sum (NULL: not stored) receives h in the
+ * residual's type, d_norm (NULL: not stored) v in norm_dtype.  d_sum may be the residual itself and
+ * d_norm x or the residual itself (same type and stride); other buffers must not overlap.  weight
+ * and bias: fp32, cols elements. */
+int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, const void* d_residual,
+                               int r_dtype, int64_t ldr, int64_t rows, int cols, int norm,
+                               const float* d_weight, const float* d_bias, float eps, void* d_sum,
+                               int64_t ldsum, void* d_norm, int norm_dtype, int64_t ldnorm,
+                               int8_t* d_q, int64_t ldq, float* d_scale, void* stream);
+
+/* out [rows][cols] = q * scale, rounded to out_dtype (1 <= cols <= 131071). */
+int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows,
+                            int cols, void* d_out, int out_dtype, int64_t ldo, void* stream);
+
+/* out[t][f] = (sum_k x[t][k] w[f][k]) * x_scale[t] * w_scale[f] + bias[f] (bias NULL: 0), x [rows]
+ * [depth] and w [features][depth] int8 rows.  The sum is exact (int32; 1 <= depth <= 131071), the
+ * rest fp32, rounded once to out_dtype. */
+int hcr_int8_linear_device(const int8_t* d_x, int64_t ldx, const float* d_x_scale, int64_t rows,
+                           const int8_t* d_w, int64_t ldw, const float* d_w_scale, int features,
+                           int depth, const float* d_bias, void* d_out, int out_dtype, int64_t ldo,
+                           void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * Fused non-LLM isRelevant combiners.  Replaces the per-node Python
