@@ -11,6 +11,7 @@
 namespace hcr {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 
 // -------------------------------------------------------------------------------------
 // Rows -> int8.  Per row: v = f(x) (below), a = max |v|, scale = a / 127,

@@ -2,6 +2,7 @@
 // Arguments are checked by the C ABI entry points; these only choose a kernel and launch it.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <cstdint>
 
 namespace hcr {
 struct I8RowArgs;

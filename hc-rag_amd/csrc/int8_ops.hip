@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include "int8_kernels.h"
+#include "int8_gemm.h"
 #include "int8_ops.h"
 #include "host_common.h"
 
@@ -36,11 +37,64 @@ int int8_rows_launch(int mode, const I8RowArgs& a, hipStream_t st) {
   return HCR_OK;
 }
 
-int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
-  const int64_t blocks = (int64_t)((a.N + 15) / 16) * ((a.T + 63) / 64);
+template <int TB, int KW>
+static int launch_direct(const I8LinearArgs& a, hipStream_t st) {
+  const int64_t blocks = (int64_t)((a.N + 15) / 16) * ((a.T + 16 * TB - 1) / (16 * TB));
   if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many outputs for one call");
-  hipLaunchKernelGGL((int8_linear_direct<4, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((int8_linear_direct<TB, KW>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
   HIPC(hipGetLastError());
+  return HCR_OK;
+}
+// 128 features x 256 tokens per workgroup of 8 waves (64 x 64 each), two workgroups per CU
+template <int OT>
+static void launch_tiles(const I8LinearArgs& a, hipStream_t st) {
+  const int nft = (a.N + 127) / 128;
+  const int tiles = nft * ((a.T + 255) / 256);
+  hipLaunchKernelGGL((int8_linear_tiles<OT, 4, 2, 4, 3, 4>), dim3((unsigned)tiles), dim3(512), 0, st, a, nft);
+}
+template <int OT>
+static void launch_stream(const I8LinearArgs& a, hipStream_t st) {
+  const int nft = (a.N + 255) / 256;
+  const unsigned tiles = (unsigned)nft * ((a.T + 255) / 256);
+  hipLaunchKernelGGL((int8_linear_stream<OT>), dim3(std::min((tiles + 7) & ~7u, 256u)), dim3(512), 0, st, a, nft, tiles);
+}
+template <int OT>
+static void launch_linear(const I8LinearArgs& a, bool stream, hipStream_t st) {
+  if (stream) launch_stream<OT>(a, st);
+  else launch_tiles<OT>(a, st);
+}
+
+// Which kernel (MI355X, us, tiles of 128 x 256 / 256 x 256 counted over the whole output):
+//   direct  below 32 tiles of 128 x 256, the workgroup's tokens as wide as leaves 256 workgroups
+//           (K = 4096, N = 1024: T = 512 20.5, tiles 31; T = 1024 38, tiles 31; K = 1024, N = 4096:
+//           T = 256 12.0, tiles 10.9; T = 512 21.6, tiles 11)
+//   stream  from 256 tiles of 256 x 256 (a tile per CU) at a depth of 1024: below, the steps between
+//           tiles weigh more than the traffic that the larger tile saves (T = 65536, N = 4096,
+//           K = 1024: 340, tiles 446; T = 65536, N = 1024, K = 4096: 257, tiles 311; T = 21853,
+//           N = 2304, K = 768: 64, tiles 58; T = 32768, N = 1152, K = 384: 34, tiles 30)
+//   tiles   otherwise
+int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
+  // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens
+  const int64_t most = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
+  const bool near = most > 0 && a.N * a.ldw <= INT32_MAX;
+  if (!near || (int64_t)((a.N + 127) / 128) * ((a.T + 255) / 256) < 32) {
+    const int64_t fb = (a.N + 15) / 16;
+    if (fb * ((a.T + 63) / 64) >= 256) return launch_direct<4, 4>(a, st);
+    if (fb * ((a.T + 31) / 32) >= 256) return launch_direct<2, 4>(a, st);
+    return launch_direct<1, 4>(a, st);
+  }
+  for (int64_t t = 0; t < a.T; t += most) {
+    I8LinearArgs c = a;
+    c.T = (int)std::min<int64_t>(most, a.T - t);
+    c.x = a.x + t * a.ldx;
+    c.sx = a.sx + t;
+    c.out = static_cast<char*>(a.out) + t * a.ldo * i8_size(a.ot);
+    const bool stream = a.K >= 1024 && (int64_t)((a.N + 255) / 256) * ((c.T + 255) / 256) >= 256;
+    if (a.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
+    else if (a.ot == HCR_BF16) launch_linear<HCR_BF16>(c, stream, st);
+    else launch_linear<HCR_F16>(c, stream, st);
+    HIPC(hipGetLastError());
+  }
   return HCR_OK;
 }
 
