@@ -23,6 +23,7 @@ def __getattr__(name):
     if name in _INT8 or name == "int8":
         import importlib
         module = importlib.import_module(".int8", __name__)
+        globals().update({n: getattr(module, n) for n in _INT8})   # found without this call from now on
         return module if name == "int8" else getattr(module, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 

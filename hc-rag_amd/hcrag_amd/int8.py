@@ -26,9 +26,23 @@ from ._lib import (HCR_ACT_GELU, HCR_ACT_NONE, HCR_BF16, HCR_F16, HCR_F32, HCR_N
 _DTYPE = {torch.float16: HCR_F16, torch.bfloat16: HCR_BF16, torch.float32: HCR_F32}
 _ACT = {"none": HCR_ACT_NONE, "gelu": HCR_ACT_GELU}
 _NORM = {"layer": HCR_NORM_LAYER, "rms": HCR_NORM_RMS}
+_I8, _F32 = torch.int8, torch.float32
+_grad_on = torch.is_grad_enabled
+_current_device = torch._C._cuda_getDevice            # (torch.cuda.current_device without its init check:
+_current_stream = torch._C._cuda_getCurrentRawStream  # the operands are device tensors; 0.1 us against 1.4)
+_new = object.__new__
 
 
-def _check(t, name: str, dtypes, dim: int, device=None) -> None:
+# A single token's call is bound by what the host does, so the checks are one expression per
+# operand; the error message is put together only when it fails.
+def _ok(t, dtypes, dim: int, device: int) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and t.get_device() == device
+            and device >= 0 and (t.shape[-1] <= 1 or t.stride(-1) == 1)
+            and not (t.requires_grad and _grad_on()))
+
+
+def _refuse(t, name: str, dtypes, dim: int, device: Optional[int] = None) -> None:
+    """Raise what is wrong with an operand that ``_ok`` turned down."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: expected a torch tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
@@ -37,27 +51,36 @@ def _check(t, name: str, dtypes, dim: int, device=None) -> None:
         raise ValueError(f"{name}: expected {dim} dimension(s), got shape {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a device tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name}: on {t.device}, other operands on {device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: elements of a row must be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name}: on {t.device}, other operands on cuda:{device}")
+    if t.requires_grad and _grad_on():
         raise ValueError(f"{name}: requires a gradient, which the int8 operators do not compute")
+    raise ValueError(f"{name}: elements of a row must be contiguous")
+
+
+def _device(t, name: str, dtypes, dim: int) -> int:
+    """The device index of a call's first operand, checked."""
+    device = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if not _ok(t, dtypes, dim, device):
+        _refuse(t, name, dtypes, dim)
+    return device
 
 
 def _ld(t) -> int:
     """Row stride in elements; of at most one row, any that its width allows."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else (cols + 15) // 16 * 16
 
 
-def _call(device, fn, *args) -> None:
+def _call(device: int, fn, *args) -> None:
     """``fn`` with torch's current stream of ``device`` as its last argument."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+    if device == _current_device():
+        rc = fn(*args, _current_stream(device))
     else:
-        with torch.cuda.device(index):
-            check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+        with torch.cuda.device(device):
+            rc = fn(*args, _current_stream(device))
+    if rc:
+        check(rc)
 
 
 class Int8Rows:
@@ -69,19 +92,22 @@ class Int8Rows:
     __slots__ = ("q", "scale")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
-        _check(q, "q", (torch.int8,), 2)
-        _check(scale, "scale", (torch.float32,), 1, q.device)
+        device = _device(q, "q", (_I8,), 2)
+        if not _ok(scale, (_F32,), 1, device):
+            _refuse(scale, "scale", (_F32,), 1, device)
         if scale.shape[0] != q.shape[0]:
             raise ValueError(f"{q.shape[0]} rows and {scale.shape[0]} scales")
-        if q.data_ptr() & 15 or _ld(q) & 15:
+        if (q.data_ptr() | _ld(q)) & 15:
             raise ValueError("q: rows must start on 16 bytes (aligned storage, row stride a multiple of 16)")
         self.q, self.scale = q, scale
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Int8Rows":
         """Uninitialised rows, laid out as the operators want them."""
-        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=device)
-        return cls(q[:, :cols], torch.empty(rows, dtype=torch.float32, device=device))
+        self = _new(cls)
+        self.q = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=_I8, device=device)
+        self.scale = torch.empty(rows, dtype=_F32, device=device)
+        return self
 
     @property
     def shape(self):
@@ -95,32 +121,33 @@ class Int8Rows:
         """[rows, cols] of the values that the rows stand for, rounded to ``dtype``."""
         if dtype not in _DTYPE:
             raise ValueError(f"dtype {dtype} is not supported here")
-        rows, cols = self.q.shape
-        out = torch.empty((rows, cols), dtype=dtype, device=self.q.device)
+        q = self.q
+        rows, cols = q.shape
+        out = torch.empty((rows, cols), dtype=dtype, device=q.device)
         if rows:
-            _call(self.q.device, lib().hcr_dequant_rows_device, self.q.data_ptr(), _ld(self.q),
-                  self.scale.data_ptr(), rows, cols, out.data_ptr(), _DTYPE[dtype], cols)
+            _call(q.get_device(), lib().hcr_dequant_rows_device, q.data_ptr(), _ld(q), self.scale.data_ptr(), rows,
+                  cols, out.data_ptr(), _DTYPE[dtype], cols)
         return out
 
 
-def _int8_out(out: Optional[Int8Rows], rows: int, cols: int, device) -> Int8Rows:
+def _int8_out(out: Optional[Int8Rows], rows: int, cols: int, like: torch.Tensor) -> Int8Rows:
     if out is None:
-        return Int8Rows.empty(rows, cols, device)
-    if tuple(out.q.shape) != (rows, cols) or out.q.device != device:
-        raise ValueError(f"out: {tuple(out.q.shape)} on {out.q.device}, expected {(rows, cols)} on {device}")
+        return Int8Rows.empty(rows, cols, like.device)
+    if tuple(out.q.shape) != (rows, cols) or out.q.device != like.device:
+        raise ValueError(f"out: {tuple(out.q.shape)} on {out.q.device}, expected {(rows, cols)} on {like.device}")
     return out
 
 
 def quantize_rows(x: torch.Tensor, act: str = "none", out: Optional[Int8Rows] = None) -> Int8Rows:
     """int8 rows of ``act(x)``; x [rows, cols] float16 / bfloat16 / float32, act "none" or "gelu"
     (exact-erf form).  Weights [features, depth] are quantised per channel by the same call."""
-    _check(x, "x", _DTYPE, 2)
+    device = _device(x, "x", _DTYPE, 2)
     if act not in _ACT:
         raise ValueError(f"unknown activation {act!r} (none | gelu)")
     rows, cols = x.shape
-    out = _int8_out(out, rows, cols, x.device)
-    _call(x.device, lib().hcr_quant_rows_device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols,
-          _ACT[act], out.q.data_ptr(), _ld(out.q), out.scale.data_ptr())
+    out = _int8_out(out, rows, cols, x)
+    _call(device, lib().hcr_quant_rows_device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols, _ACT[act],
+          out.q.data_ptr(), _ld(out.q), out.scale.data_ptr())
     return out
 
 
@@ -136,36 +163,49 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     quantised.  sum_out may be the residual itself, norm_out x or the residual itself; other
     operands must not overlap.
     """
-    _check(x, "x", _DTYPE, 2)
+    device = _device(x, "x", _DTYPE, 2)
     if norm not in _NORM:
         raise ValueError(f"unknown norm {norm!r} (layer | rms)")
-    rows, cols = x.shape
-    dev = x.device
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None or name == "weight":
-            _check(t, name, (torch.float32,), 1, dev)
-            if t.shape[0] != cols:
-                raise ValueError(f"{name}: {t.shape[0]} elements, expected {cols}")
-    for t, name in ((residual, "residual"), (sum_out, "sum_out"), (norm_out, "norm_out")):
-        if t is not None:
-            _check(t, name, _DTYPE, 2, dev)
-            if t.shape != x.shape:
-                raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {(rows, cols)}")
-    if sum_out is not None and (residual is None or sum_out.dtype != residual.dtype):
-        raise ValueError("sum_out needs a residual of the same dtype")
-    out = _int8_out(out, rows, cols, dev)
-    _call(dev, lib().hcr_norm_quant_rows_device, x.data_ptr(), _DTYPE[x.dtype], _ld(x),
-          residual.data_ptr() if residual is not None else None,
-          _DTYPE[residual.dtype] if residual is not None else HCR_F32,
-          _ld(residual) if residual is not None else 0, rows, cols, _NORM[norm],
-          weight.data_ptr(), bias.data_ptr() if bias is not None else None, eps,
-          sum_out.data_ptr() if sum_out is not None else None,
-          _ld(sum_out) if sum_out is not None else 0,
-          norm_out.data_ptr() if norm_out is not None else None,
-          _DTYPE[norm_out.dtype] if norm_out is not None else HCR_F32,
-          _ld(norm_out) if norm_out is not None else 0,
+    shape = x.shape
+    rows, cols = shape
+    if not _ok(weight, (_F32,), 1, device):
+        _refuse(weight, "weight", (_F32,), 1, device)
+    if weight.shape[0] != cols:
+        raise ValueError(f"weight: {weight.shape[0]} elements, expected {cols}")
+    bias_p = resid_p = sum_p = norm_p = None
+    resid_t = norm_t = HCR_F32
+    resid_ld = sum_ld = norm_ld = 0
+    if bias is not None:
+        if not _ok(bias, (_F32,), 1, device):
+            _refuse(bias, "bias", (_F32,), 1, device)
+        if bias.shape[0] != cols:
+            raise ValueError(f"bias: {bias.shape[0]} elements, expected {cols}")
+        bias_p = bias.data_ptr()
+    if residual is not None:
+        resid_t, resid_ld = _rows_operand(residual, "residual", shape, device)
+        resid_p = residual.data_ptr()
+    if sum_out is not None:
+        if residual is None or sum_out.dtype != residual.dtype:
+            raise ValueError("sum_out needs a residual of the same dtype")
+        _, sum_ld = _rows_operand(sum_out, "sum_out", shape, device)
+        sum_p = sum_out.data_ptr()
+    if norm_out is not None:
+        norm_t, norm_ld = _rows_operand(norm_out, "norm_out", shape, device)
+        norm_p = norm_out.data_ptr()
+    out = _int8_out(out, rows, cols, x)
+    _call(device, lib().hcr_norm_quant_rows_device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), resid_p, resid_t, resid_ld,
+          rows, cols, _NORM[norm], weight.data_ptr(), bias_p, eps, sum_p, sum_ld, norm_p, norm_t, norm_ld,
           out.q.data_ptr(), _ld(out.q), out.scale.data_ptr())
     return out
+
+
+def _rows_operand(t, name: str, shape, device: int):
+    """(dtype, row stride) of a [rows, cols] operand of a floating type."""
+    if not _ok(t, _DTYPE, 2, device):
+        _refuse(t, name, _DTYPE, 2, device)
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return _DTYPE[t.dtype], _ld(t)
 
 
 def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
@@ -174,28 +214,31 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
     [rows, features] in ``dtype`` (or into ``out``).  The integer sums are exact."""
     if not isinstance(x, Int8Rows) or not isinstance(w, Int8Rows):
         raise ValueError("x and w: expected Int8Rows (quantize_rows makes them)")
-    rows, depth = x.q.shape
-    features = w.q.shape[0]
-    dev = x.q.device
-    if w.q.shape[1] != depth:
-        raise ValueError(f"x has depth {depth}, w {w.q.shape[1]}")
-    if w.q.device != dev:
-        raise ValueError(f"w: on {w.q.device}, x on {dev}")
+    xq, wq = x.q, w.q
+    rows, depth = xq.shape
+    features, depth_w = wq.shape
+    device = xq.get_device()
+    if depth_w != depth:
+        raise ValueError(f"x has depth {depth}, w {depth_w}")
+    if wq.get_device() != device:
+        raise ValueError(f"w: on {wq.device}, x on {xq.device}")
+    bias_p = None
     if bias is not None:
-        _check(bias, "bias", (torch.float32,), 1, dev)
+        if not _ok(bias, (_F32,), 1, device):
+            _refuse(bias, "bias", (_F32,), 1, device)
         if bias.shape[0] != features:
             raise ValueError(f"bias: {bias.shape[0]} elements, expected {features}")
+        bias_p = bias.data_ptr()
     if out is None:
-        if dtype not in _DTYPE:
+        code = _DTYPE.get(dtype)
+        if code is None:
             raise ValueError(f"dtype {dtype} is not supported here")
-        out = torch.empty((rows, features), dtype=dtype, device=dev)
+        out = torch.empty((rows, features), dtype=dtype, device=xq.device)
+        ldo = features
     else:
-        _check(out, "out", _DTYPE, 2, dev)
-        if tuple(out.shape) != (rows, features):
-            raise ValueError(f"out: shape {tuple(out.shape)}, expected {(rows, features)}")
-    _call(dev, lib().hcr_int8_linear_device, x.q.data_ptr(), _ld(x.q), x.scale.data_ptr(), rows,
-          w.q.data_ptr(), _ld(w.q), w.scale.data_ptr(), features, depth,
-          bias.data_ptr() if bias is not None else None, out.data_ptr(), _DTYPE[out.dtype], _ld(out))
+        code, ldo = _rows_operand(out, "out", (rows, features), device)
+    _call(device, lib().hcr_int8_linear_device, xq.data_ptr(), _ld(xq), x.scale.data_ptr(), rows, wq.data_ptr(),
+          _ld(wq), w.scale.data_ptr(), features, depth, bias_p, out.data_ptr(), code, ldo)
     return out
 
 
