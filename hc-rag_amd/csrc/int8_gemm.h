@@ -64,8 +64,6 @@ __device__ __forceinline__ void i8_lds_read_tx(uint32_t a, float (&t)[4]) {
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, char* lds_dst, int voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds_dst, 4, voff, soff, 0, 0);
 }
-template <typename T>
-__device__ __forceinline__ uint32_t i8_pack2(float x, float y) { return i8_bits16<T>(x) | i8_bits16<T>(y) << 16; }
 
 // f(integral_constant<int, 0>) .. f(integral_constant<int, N - 1>): a descriptor picked by a loop
 // index rather than a constant ends up in memory and is read back lane by lane

@@ -5,7 +5,6 @@
 //   int8_linear_direct    y = x . w^T of int8 rows, few tokens
 #pragma once
 #include "device_common.h"
-#include "gelu.h"
 #include "hcrag.h"
 
 namespace hcr {
@@ -41,135 +40,181 @@ struct I8RowArgs {
   int cols;
   float eps;
   int xt, rt, yt;                  // hcr_dtype of x, r (and sum), y
-  int vec;                         // every row of x, r, sum, y, g, b starts on 16 bytes
 };
 
-struct I8Raw { uint4 a, b; };      // 8 elements as loaded: 16-bit types in a, f32 in a and b
-
-// elements [i, i + 8) of a row, n of them in the row (n >= 8: whole chunk)
-__device__ __forceinline__ void i8_load(I8Raw& o, const char* row, bool f32, int i, int n, bool vec) {
-  if (vec && n >= 8) {
-    if (f32) {
-      const uint4* p = reinterpret_cast<const uint4*>(row + (size_t)i * 4);
-      o.a = p[0];
-      o.b = p[1];
-    } else {
-      o.a = *reinterpret_cast<const uint4*>(row + (size_t)i * 2);
-    }
-    return;
-  }
-  uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-  if (f32) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) if (e < n) w[e] = reinterpret_cast<const uint32_t*>(row)[i + e];
-    o.b = uint4{w[4], w[5], w[6], w[7]};
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) w[e >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(row)[i + e] << (16 * (e & 1));
-  }
-  o.a = uint4{w[0], w[1], w[2], w[3]};
+// gelu(x) = x Phi(x) = x / (1 + 2^-z), z = log2(Phi / (1 - Phi)) = x g(x^2): g as a polynomial fitted so
+// that Phi is within 2.9e-8 everywhere (its last coefficient is positive: z keeps x's sign past the
+// fit, where Phi is 0 or 1).  7 instructions fewer per element than erf_as's form, whose division
+// comes on top of a longer polynomial: the activation's kernel is bound by arithmetic.  In fp32
+// |dv| <= 0.4 (1.6e-7 |x| + 2.4e-7 |v|).
+__device__ __forceinline__ float i8_gelu(float x) {
+  const float t = x * x;
+  float g = 5.067230635091846e-09f;
+  g = fmaf(g, t, -3.816310822912783e-07f);
+  g = fmaf(g, t, 1.1439830814197194e-05f);
+  g = fmaf(g, t, -1.5957992582116276e-04f);
+  g = fmaf(g, t, -9.4049253675621e-05f);
+  g = fmaf(g, t, 1.0483512282371521e-01f);
+  g = fmaf(g, t, 2.3022093772888184e+00f);
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-(g * x)));
 }
-__device__ __forceinline__ void i8_convert(float (&v)[8], const I8Raw& o, int type) {
-  const uint32_t w[8] = {o.a.x, o.a.y, o.a.z, o.a.w, o.b.x, o.b.y, o.b.z, o.b.w};
-  if (type == HCR_F32) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
-  } else if (type == HCR_BF16) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float((e & 1) ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
-  } else {
+
+// v inv, rounded, plus 1.5 * 2^23, rounded: the low byte is v inv to the nearest whole number, ties to
+// even.  (Not as one fma: q is defined by the rounded product.)
+__device__ __forceinline__ uint32_t i8_step(float v, float inv) {
+#pragma clang fp contract(off)
+  const float p = v * inv;
+  return __float_as_uint(p + 12582912.f);
+}
+
+// 16 bytes at any alignment: one instruction, the hardware takes unaligned vectors (rows of odd
+// widths, 65521 x 1531 bf16: 139 us element by element).
+typedef uint32_t uintx4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ uintx4 i8_load16(const char* p) { return *reinterpret_cast<const uintx4_any*>(p); }
+__device__ __forceinline__ void i8_store16(char* p, uintx4 u) { *reinterpret_cast<uintx4_any*>(p) = u; }
+
+struct I8Raw { uintx4 a, b; };     // 8 elements as loaded: 16-bit types in a, f32 in a and b
+
+// elements [i, i + 8) of a row of cols: whole chunks as vectors, the row's last, partial one element
+// by element (the row's last element again past its end: the caller drops those)
+template <bool F32>
+__device__ __forceinline__ void i8_load(I8Raw& o, const char* row, int i, int cols) {
+  if (i + 8 <= cols) {
+    const char* p = row + (int64_t)i * (F32 ? 4 : 2);
+    o.a = i8_load16(p);
+    if constexpr (F32) o.b = i8_load16(p + 16);
+  } else if (i < cols) {
+    uint32_t w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-      v[e] = (float)__builtin_bit_cast(_Float16, h);
+      const int j = min(i + e, cols - 1);
+      w[e] = F32 ? reinterpret_cast<const uint32_t*>(row)[j] : reinterpret_cast<const uint16_t*>(row)[j];
+    }
+    if constexpr (F32) {
+      o.a = uintx4{w[0], w[1], w[2], w[3]};
+      o.b = uintx4{w[4], w[5], w[6], w[7]};
+    } else {
+      o.a = uintx4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
+    }
+  }
+}
+__device__ __forceinline__ void i8_convert(float (&v)[8], const I8Raw& o, int type) {
+  if (type == HCR_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = __uint_as_float(o.a[e]); v[4 + e] = __uint_as_float(o.b[e]); }
+  } else if (type == HCR_BF16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(o.a[e] << 16);
+      v[2 * e + 1] = __uint_as_float(o.a[e] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)o.a[e]);
+      v[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(o.a[e] >> 16));
     }
   }
 }
 template <typename T>
 __device__ __forceinline__ uint32_t i8_bits16(float v) { return __builtin_bit_cast(uint16_t, (T)v); }
-__device__ __forceinline__ void i8_store(char* row, int type, int i, int n, bool vec, const float (&v)[8]) {
+template <typename T>
+__device__ __forceinline__ uint32_t i8_pack2(float x, float y) { return i8_bits16<T>(x) | i8_bits16<T>(y) << 16; }
+// elements [i, i + 8) of a row of cols, those that exist
+__device__ __forceinline__ void i8_store(char* row, int type, int i, int cols, const float (&v)[8]) {
   if (type == HCR_F32) {
-    float* p = reinterpret_cast<float*>(row) + i;
-    if (vec && n >= 8) {
-      reinterpret_cast<float4*>(p)[0] = float4{v[0], v[1], v[2], v[3]};
-      reinterpret_cast<float4*>(p)[1] = float4{v[4], v[5], v[6], v[7]};
+    char* p = row + (int64_t)i * 4;
+    if (i + 8 <= cols) {
+      i8_store16(p, uintx4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+      i8_store16(p + 16, uintx4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])});
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) if (e < n) p[e] = v[e];
+      for (int e = 0; e < 7; ++e) if (i + e < cols) reinterpret_cast<float*>(p)[e] = v[e];
     }
     return;
   }
-  uint32_t h[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = type == HCR_BF16 ? i8_bits16<__bf16>(v[e]) : i8_bits16<_Float16>(v[e]);
-  uint16_t* p = reinterpret_cast<uint16_t*>(row) + i;
-  if (vec && n >= 8) {
-    *reinterpret_cast<uint4*>(p) = uint4{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
+  uintx4 h;
+  if (type == HCR_BF16) h = uintx4{i8_pack2<__bf16>(v[0], v[1]), i8_pack2<__bf16>(v[2], v[3]), i8_pack2<__bf16>(v[4], v[5]), i8_pack2<__bf16>(v[6], v[7])};
+  else h = uintx4{i8_pack2<_Float16>(v[0], v[1]), i8_pack2<_Float16>(v[2], v[3]), i8_pack2<_Float16>(v[4], v[5]), i8_pack2<_Float16>(v[6], v[7])};
+  char* p = row + (int64_t)i * 2;
+  if (i + 8 <= cols) {
+    i8_store16(p, h);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) if (e < n) p[e] = (uint16_t)h[e];
+    for (int e = 0; e < 7; ++e)
+      if (i + e < cols) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(h[e >> 1] >> (16 * (e & 1)));
   }
 }
 
-// sum / maximum over the WAVES waves that share a row (WAVES == 1: each wave has its own row)
-template <int WAVES>
-__device__ __forceinline__ float i8_row_sum(float s, float* red, int wave, int lane) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+// Reductions over the WAVES waves that share a row (WAVES == 1: each wave has its own row), the same
+// result in every lane.  Within 16 lanes by DPP, over the rest by lane swaps: no LDS round trips.
+template <int CTRL>
+__device__ __forceinline__ uint32_t i8_dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <typename F>
+__device__ __forceinline__ uint32_t i8_wave_reduce(uint32_t v, F f) {
+  v = f(v, i8_dpp<0xB1>(v));       // quad_perm [1 0 3 2]
+  v = f(v, i8_dpp<0x4E>(v));       // quad_perm [2 3 0 1]
+  v = f(v, i8_dpp<0x141>(v));      // mirrored in 8 lanes
+  v = f(v, i8_dpp<0x140>(v));      // mirrored in 16 lanes
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = f(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f(b[0], b[1]);
+}
+template <int WAVES, typename F>
+__device__ __forceinline__ uint32_t i8_row_reduce(uint32_t v, uint32_t* red, int wave, int lane, F f) {
+  v = i8_wave_reduce(v, f);
   if constexpr (WAVES > 1) {
     __syncthreads();               // (the previous reduction's reads of red are done)
-    if (lane == 0) red[wave] = s;
+    if (lane == 0) red[wave] = v;
     __syncthreads();
-    s = 0.f;
+    v = red[0];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += red[w];
+    for (int w = 1; w < WAVES; ++w) v = f(v, red[w]);
   }
-  return s;
+  return v;
 }
 template <int WAVES>
-__device__ __forceinline__ uint32_t i8_row_max(uint32_t s, float* red, int wave, int lane) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) s = max(s, (uint32_t)__shfl_xor((int)s, m, 64));
-  if constexpr (WAVES > 1) {
-    __syncthreads();
-    if (lane == 0) red[wave] = __uint_as_float(s);
-    __syncthreads();
-    s = 0u;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) s = max(s, __float_as_uint(red[w]));
-  }
-  return s;
+__device__ __forceinline__ float i8_row_sum(float s, uint32_t* red, int wave, int lane) {
+  return __uint_as_float(i8_row_reduce<WAVES>(__float_as_uint(s), red, wave, lane, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 
 // One row per WAVES waves; WAVES == 1 puts 4 rows in a workgroup.  Covers cols <= 512 WAVES NCH.
 template <int MODE, int WAVES, int NCH>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 rows_to_int8_kernel(I8RowArgs a) {
-  __shared__ float red[WAVES > 1 ? WAVES : 1];
+  __shared__ uint32_t red[WAVES > 1 ? WAVES : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
   if (WAVES == 1 && row >= a.rows) return;
   const int tid = WAVES == 1 ? lane : threadIdx.x;
   constexpr int NTH = 64 * WAVES;
   constexpr bool NORM = MODE == I8_LAYER || MODE == I8_RMS;
-  const bool vec = a.vec != 0;
   const bool x32 = a.xt == HCR_F32, r32 = a.rt == HCR_F32;
   const char* xr = reinterpret_cast<const char*>(a.x) + row * a.ldx * (x32 ? 4 : 2);
   const char* rr = reinterpret_cast<const char*>(a.r) + row * a.ldr * (r32 ? 4 : 2);
   I8Raw xs[NCH], rs[NORM ? NCH : 1];
+  // (one branch on the element size around all of a row's loads: they are in flight together)
+  if (x32) {
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int i = (tid + NTH * c) * 8;
-    xs[c] = I8Raw{};
-    if (i < a.cols) i8_load(xs[c], xr, x32, i, a.cols - i, vec);
+    for (int c = 0; c < NCH; ++c) i8_load<true>(xs[c], xr, (tid + NTH * c) * 8, a.cols);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) i8_load<false>(xs[c], xr, (tid + NTH * c) * 8, a.cols);
   }
   if constexpr (NORM) {
+    if (a.r) {
+      if (r32) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      const int i = (tid + NTH * c) * 8;
-      rs[c] = I8Raw{};
-      if (a.r && i < a.cols) i8_load(rs[c], rr, r32, i, a.cols - i, vec);
+        for (int c = 0; c < NCH; ++c) i8_load<true>(rs[c], rr, (tid + NTH * c) * 8, a.cols);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) i8_load<false>(rs[c], rr, (tid + NTH * c) * 8, a.cols);
+      }
     }
   }
   float v[NCH][8];                 // (elements past the row's end are 0)
@@ -186,7 +231,12 @@ rows_to_int8_kernel(I8RowArgs a) {
     }
     if constexpr (MODE == I8_GELU) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c][e] = gelu_erf(v[c][e]);
+      for (int e = 0; e < 8; ++e) v[c][e] = i8_gelu(v[c][e]);
+    }
+    const int n = a.cols - (tid + NTH * c) * 8;
+    if (n < 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = e < n ? v[c][e] : 0.f;
     }
   }
   bool overflow = false;
@@ -203,11 +253,15 @@ rows_to_int8_kernel(I8RowArgs a) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int n = a.cols - (tid + NTH * c) * 8;
+      float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = e < n ? v[c][e] - mean : 0.f;
-        s = fmaf(d, d, s);
+      for (int e = 0; e < 8; ++e) d[e] = v[c][e] - mean;
+      if (n < 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = e < n ? d[e] : 0.f;
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf(d[e], d[e], s);
     }
     const float var = i8_row_sum<WAVES>(s, red, wave, lane) / (float)a.cols;
     overflow = !(var < INFINITY);  // the squares left fp32's range: the row is not representable
@@ -217,7 +271,7 @@ rows_to_int8_kernel(I8RowArgs a) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int i = (tid + NTH * c) * 8;
-        if (i < a.cols) i8_store(sr, a.rt, i, a.cols - i, vec, v[c]);
+        if (i < a.cols) i8_store(sr, a.rt, i, a.cols, v[c]);
       }
     }
 #pragma unroll
@@ -226,30 +280,43 @@ rows_to_int8_kernel(I8RowArgs a) {
       if (n <= 0) continue;
       I8Raw raw;
       float g[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      i8_load(raw, reinterpret_cast<const char*>(a.g), true, i, n, vec);
+      i8_load<true>(raw, reinterpret_cast<const char*>(a.g), i, a.cols);
       i8_convert(g, raw, HCR_F32);
       if (a.b) {
-        i8_load(raw, reinterpret_cast<const char*>(a.b), true, i, n, vec);
+        i8_load<true>(raw, reinterpret_cast<const char*>(a.b), i, a.cols);
         i8_convert(b, raw, HCR_F32);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c][e] = e < n ? fmaf((v[c][e] - mean) * rstd, g[e], b[e]) : 0.f;
+      for (int e = 0; e < 8; ++e) v[c][e] = fmaf((v[c][e] - mean) * rstd, g[e], b[e]);
+      if (n < 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[c][e] = e < n ? v[c][e] : 0.f;
+      }
     }
     if (a.y) {
       char* yr = reinterpret_cast<char*>(a.y) + row * a.ldy * (a.yt == HCR_F32 ? 4 : 2);
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int i = (tid + NTH * c) * 8;
-        if (i < a.cols) i8_store(yr, a.yt, i, a.cols - i, vec, v[c]);
+        if (i < a.cols) i8_store(yr, a.yt, i, a.cols, v[c]);
       }
     }
   }
-  uint32_t m = overflow ? 0x7FC00000u : 0u;
+  // the largest pattern as signed (of the positive elements) and as unsigned (of the negative ones,
+  // if there are any): one three-way maximum per two elements each
+  int mp = 0;
+  uint32_t mn = 0u;
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[c][e]) & 0x7FFFFFFFu);
-  m = i8_row_max<WAVES>(m, red, wave, lane);
+    for (int e = 0; e < 8; e += 2) {
+      const uint32_t u0 = __float_as_uint(v[c][e]), u1 = __float_as_uint(v[c][e + 1]);
+      mp = max(max(mp, (int)u0), (int)u1);
+      mn = max(max(mn, u0), u1);
+    }
+  uint32_t m = max((uint32_t)mp, (mn >> 31) ? mn & 0x7FFFFFFFu : 0u);
+  if (overflow) m = 0x7FC00000u;
+  m = i8_row_reduce<WAVES>(m, red, wave, lane, [](uint32_t p, uint32_t q) { return max(p, q); });
   const float amax = __uint_as_float(m);
   const bool bad = m >= 0x7F800000u;
   const bool zero = bad || amax < 0x1p-100f;
@@ -260,23 +327,29 @@ rows_to_int8_kernel(I8RowArgs a) {
   for (int c = 0; c < NCH; ++c) {
     const int i = (tid + NTH * c) * 8, n = a.cols - i;
     if (n <= 0) continue;
-    uint32_t w[2] = {0u, 0u};
+    // |v inv| <= 127 (1 + 2^-23), which rounds to 127; two's complement in the low byte (bad and
+    // zero rows: 0 whatever v is)
+    uint32_t u[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // (|v inv| <= 127 (1 + 2^-23), which rounds to 127; bad and zero rows are 0 whatever v is)
-      const int qe = zero ? 0 : (int)rintf(v[c][e] * inv);
-      w[e >> 2] |= ((uint32_t)qe & 255u) << (8 * (e & 3));
+    for (int e = 0; e < 8; ++e) u[e] = i8_step(v[c][e], inv);
+    uint32_t w[2];
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const uint32_t lo = __builtin_amdgcn_perm(u[4 * d + 1], u[4 * d], 0x0C0C0400u);
+      const uint32_t hi = __builtin_amdgcn_perm(u[4 * d + 3], u[4 * d + 2], 0x0C0C0400u);
+      w[d] = zero ? 0u : lo | hi << 16;
     }
     if (n >= 8) *reinterpret_cast<uint2*>(qr + i) = uint2{w[0], w[1]};   // (q rows start on 16 bytes)
     else
-      for (int e = 0; e < n; ++e) qr[i + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
+#pragma unroll
+      for (int e = 0; e < 7; ++e) if (e < n) qr[i + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
   }
 }
 
 // out = q * scale, rounded once to the output's type.  One thread per 8 elements.
 __global__ void __launch_bounds__(256)
 int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t rows,
-                    int cols, void* __restrict__ out, int ot, int64_t ldo, int vec) {
+                    int cols, void* __restrict__ out, int ot, int64_t ldo) {
   const int per = (cols + 7) >> 3;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = id / per;
@@ -294,7 +367,7 @@ int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __re
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * s;
-  i8_store(reinterpret_cast<char*>(out) + row * ldo * (ot == HCR_F32 ? 4 : 2), ot, i, n, vec != 0, v);
+  i8_store(reinterpret_cast<char*>(out) + row * ldo * (ot == HCR_F32 ? 4 : 2), ot, i, cols, v);
 }
 
 // -------------------------------------------------------------------------------------

@@ -18,13 +18,18 @@ static void launch_rows(const I8RowArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((rows_to_int8_kernel<MODE, WAVES, NCH>), dim3(grid), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0,
                      st, a);
 }
+// The narrowest layout that holds a row.  Up to 2048 columns a wave per row (a workgroup per row
+// pays its barriers three times: 60000 x 384 LayerNorm 45 us, 89 with 4 waves a row; 65536 x 2048
+// RMS 172, 184), above that 2 chunks per thread (30000 x 8192 RMS 313 us, 349 with 4 waves x 4 chunks,
+// 416 with 16 x 1; 20000 x 16384: 449, 493 with 16 x 4).
 template <int MODE>
 static void launch_rows_mode(const I8RowArgs& a, hipStream_t st) {
   if (a.cols <= 512) launch_rows<MODE, 1, 1>(a, st);
   else if (a.cols <= 1024) launch_rows<MODE, 1, 2>(a, st);
   else if (a.cols <= 2048) launch_rows<MODE, 1, 4>(a, st);
   else if (a.cols <= 4096) launch_rows<MODE, 4, 2>(a, st);
-  else if (a.cols <= 8192) launch_rows<MODE, 4, 4>(a, st);
+  else if (a.cols <= 8192) launch_rows<MODE, 8, 2>(a, st);
+  else if (a.cols <= 16384) launch_rows<MODE, 16, 2>(a, st);
   else launch_rows<MODE, 16, 4>(a, st);
 }
 
@@ -122,9 +127,6 @@ static int check_rows(int64_t rows, int cols, int64_t max_cols) {
   if (cols < 1 || cols > max_cols) return hcr_set_errorf(HCR_EINVAL, "cols must be in [1, %lld], got %d", (long long)max_cols, cols);
   return HCR_OK;
 }
-// rows that start on 16 bytes, so that whole chunks of 8 elements are aligned vectors
-static bool rows_on16(const void* p, int dt, int64_t ld) { return on(p, 16) && ld * (int64_t)float_size(dt) % 16 == 0; }
-
 extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int cols, int act,
                                      int8_t* d_q, int64_t ldq, float* d_scale, void* stream) {
   CHECK(check_rows(rows, cols, kI8MaxRowCols));
@@ -137,7 +139,6 @@ extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, 
   I8RowArgs a{};
   a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
   a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = cols;
-  a.vec = rows_on16(d_x, x_dtype, ldx);
   return int8_rows_launch(act == HCR_ACT_GELU ? I8_GELU : I8_QUANT, a, (hipStream_t)stream);
 }
 
@@ -166,9 +167,6 @@ extern "C" int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t 
   a.y = d_norm; a.ldy = ldnorm; a.yt = norm_dtype;
   a.g = d_weight; a.b = d_bias; a.eps = eps;
   a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = cols;
-  a.vec = rows_on16(d_x, x_dtype, ldx) && on(d_weight, 16) && on(d_bias, 16) &&
-          (!d_residual || rows_on16(d_residual, r_dtype, ldr)) && (!d_sum || rows_on16(d_sum, r_dtype, ldsum)) &&
-          (!d_norm || rows_on16(d_norm, norm_dtype, ldnorm));
   return int8_rows_launch(norm == HCR_NORM_LAYER ? I8_LAYER : I8_RMS, a, (hipStream_t)stream);
 }
 
@@ -183,7 +181,7 @@ extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const flo
   const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
   if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many elements for one call");
   hipLaunchKernelGGL(int8_to_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, ldq,
-                     d_scale, rows, cols, d_out, out_dtype, ldo, rows_on16(d_out, out_dtype, ldo) ? 1 : 0);
+                     d_scale, rows, cols, d_out, out_dtype, ldo);
   HIPC(hipGetLastError());
   return HCR_OK;
 }
