@@ -346,28 +346,30 @@ rows_to_int8_kernel(I8RowArgs a) {
   }
 }
 
-// out = q * scale, rounded once to the output's type.  One thread per 8 elements.
+// out = q * scale, rounded once to the output's type.  One thread per 8 elements; the last 8 of a row
+// that is no multiple of 8 overlap the ones before (the same values are stored twice).
 __global__ void __launch_bounds__(256)
-int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t rows,
+int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, unsigned rows,
                     int cols, void* __restrict__ out, int ot, int64_t ldo) {
-  const int per = (cols + 7) >> 3;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / per;
+  const unsigned per = (unsigned)(cols + 7) >> 3;
+  const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const unsigned row = id >> 32 ? (unsigned)(id / per) : (unsigned)id / per;   // (the 64-bit one is long)
   if (row >= rows) return;
-  const int i = (int)(id - row * per) * 8, n = cols - i;
-  uint32_t w[2] = {0u, 0u};
+  const int i = min((int)(unsigned)(id - (uint64_t)row * per) * 8, max(cols - 8, 0));
   const int8_t* qr = q + row * ldq + i;
-  if (n >= 8) {
-    const uint2 u = *reinterpret_cast<const uint2*>(qr);
-    w[0] = u.x; w[1] = u.y;
-  } else {
-    for (int e = 0; e < n; ++e) w[e >> 2] |= (uint32_t)(uint8_t)qr[e] << (8 * (e & 3));
-  }
+  char* orow = reinterpret_cast<char*>(out) + row * ldo * (ot == HCR_F32 ? 4 : 2);
   const float s = scale[row];
   float v[8];
+  if (cols >= 8) {
+    typedef uint32_t uintx2_any __attribute__((ext_vector_type(2), aligned(1)));
+    const uintx2_any w = *reinterpret_cast<const uintx2_any*>(qr);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * s;
-  i8_store(reinterpret_cast<char*>(out) + row * ldo * (ot == HCR_F32 ? 4 : 2), ot, i, cols, v);
+    for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * s;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)qr[min(e, cols - 1)] * s;
+  }
+  i8_store(orow, ot, i, cols, v);
 }
 
 // -------------------------------------------------------------------------------------

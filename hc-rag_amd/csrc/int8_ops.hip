@@ -181,7 +181,7 @@ extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const flo
   const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
   if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many elements for one call");
   hipLaunchKernelGGL(int8_to_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, ldq,
-                     d_scale, rows, cols, d_out, out_dtype, ldo);
+                     d_scale, (unsigned)rows, cols, d_out, out_dtype, ldo);
   HIPC(hipGetLastError());
   return HCR_OK;
 }
