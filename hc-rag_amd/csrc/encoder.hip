@@ -13,7 +13,9 @@
 //   HCR_F32             reference precision (the reference encodes in fp32 torch,
 //                       experiments/embedding_generator.py:124): every projection GEMM as the
 //                       three-term split-f16 product on the same MFMA kernel (~22-bit operands,
-//                       fp32 accumulation), fp32 attention, library erff / expf.
+//                       fp32 accumulation), fp32 attention, library erff / expf;
+//   HCR_I8              the projections as int8 products (int8_ops.hip): LayerNorms, GELU and
+//                       attention leave int8 rows with a scale each, the products f16.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,6 +29,8 @@
 #include "gemm_v4.h"
 #define HCR_TOPK_TEMPLATES_ONLY   // (gemm_ws.h reaches topk_kernels.h: its kernels live in hcrag_index.hip)
 #include "gemm_ws.h"
+#include "int8_args.h"
+#include "int8_ops.h"
 #include "hcrag.h"
 #include "host_common.h"
 
@@ -37,6 +41,7 @@ struct EncLayer {
   // GEMM output scales (reference-precision mode: undo the weights' power-of-two scale and
   // the split's 2^11; 1 in the fast modes)
   float sqkv = 1.f, so = 1.f, si = 1.f, so2 = 1.f;
+  DevBuf cqkv, co, ci, co2;      // HCR_I8: the weights' scale per output channel
 };
 
 // One sub-batch's activations and the stream its layers run on (hcr_encode_device splits a
@@ -45,6 +50,7 @@ struct EncLayer {
 struct EncWork {
   DevBuf x, xh, qkv, ctx, inter, y;
   DevBuf pk_off, pk_map, pk_ok, pk_tot;   // token packing (pack_tokens_kernel)
+  DevBuf q8, s8;                          // HCR_I8: the int8 rows under way and their scales
   DevBuf split_ws, split_cnt;             // split GEMM last-round K-split: chunk slabs and a
                                           // ticket counter per tile (zeroed once, reset by use)
   hipStream_t st = nullptr;               // (split sub-batches only; the first runs unsplit
@@ -53,7 +59,7 @@ struct EncWork {
                                           // other sub-batch's stream fills the partly filled
                                           // last rounds (reference-precision mode, r06)
   void release() {
-    DevBuf* b[] = {&x, &xh, &qkv, &ctx, &inter, &y, &pk_off, &pk_map, &pk_ok, &pk_tot, &split_ws, &split_cnt};
+    DevBuf* b[] = {&x, &xh, &qkv, &ctx, &inter, &y, &pk_off, &pk_map, &pk_ok, &pk_tot, &q8, &s8, &split_ws, &split_cnt};
     for (DevBuf* d : b) d->release();
   }
 };
@@ -128,8 +134,10 @@ extern "C" int hcr_encoder_create(int device, const hcr_bert_config* cfg, int co
   if (c.layers <= 0 || c.vocab_size <= 0 || c.max_position <= 0 || c.type_vocab <= 0)
     return hcr_set_error(HCR_EINVAL, "bad config sizes");
   if (c.pooling != 0 && c.pooling != 1) return hcr_set_error(HCR_EINVAL, "pooling must be 0 (mean) or 1 (cls)");
-  if (compute_dtype != HCR_F16 && compute_dtype != HCR_BF16 && compute_dtype != HCR_F32)
-    return hcr_set_error(HCR_EINVAL, "compute dtype must be HCR_F16, HCR_BF16 or HCR_F32");
+  if (compute_dtype != HCR_F16 && compute_dtype != HCR_BF16 && compute_dtype != HCR_F32 && compute_dtype != HCR_I8)
+    return hcr_set_error(HCR_EINVAL, "compute dtype must be HCR_F16, HCR_BF16, HCR_F32 or HCR_I8");
+  if (compute_dtype == HCR_I8 && c.intermediate > kI8MaxRowCols)
+    return hcr_set_errorf(HCR_EINVAL, "HCR_I8 needs intermediate <= %d, got %d", kI8MaxRowCols, c.intermediate);
   int ndev = 0;
   if (hipGetDeviceCount(&ndev) != hipSuccess) ndev = 0;
   if (device < 0 || device >= ndev)
@@ -164,7 +172,7 @@ extern "C" int hcr_encoder_destroy(hcr_encoder* e) {
   }
   if (e->ev_in) (void)hipEventDestroy(e->ev_in);
   for (auto& L : e->layers) {
-    DevBuf* lb[] = {&L.wqkv, &L.bqkv, &L.wo, &L.bo, &L.ln1g, &L.ln1b, &L.wi, &L.bi, &L.wo2, &L.bo2, &L.ln2g, &L.ln2b};
+    DevBuf* lb[] = {&L.wqkv, &L.bqkv, &L.wo, &L.bo, &L.ln1g, &L.ln1b, &L.wi, &L.bi, &L.wo2, &L.bo2, &L.ln2g, &L.ln2b, &L.cqkv, &L.co, &L.ci, &L.co2};
     for (DevBuf* b : lb) b->release();
   }
   if (e->stream) (void)hipStreamDestroy(e->stream);
@@ -223,6 +231,28 @@ static int upload_weights(DevBuf& dst, const std::vector<float>& src, int64_t ro
   return HCR_OK;
 }
 
+// HCR_I8: projection weights [rows][cols] fp32 -> int8 rows, a scale per row (output channel).
+static int upload_weights_i8(DevBuf& dst, DevBuf& scale, const std::vector<float>& src, int64_t rows, int cols,
+                             hipStream_t st) {
+  CHECK(dst.ensure((size_t)rows * cols));
+  CHECK(scale.ensure((size_t)rows * 4));
+  DevBuf tmp;
+  int rc = tmp.ensure((size_t)rows * cols * 4);
+  if (rc == HCR_OK) {
+    hipError_t he = hipMemcpyAsync(tmp.p, src.data(), (size_t)rows * cols * 4, hipMemcpyHostToDevice, st);
+    I8RowArgs a{};
+    a.x = tmp.p; a.ldx = cols; a.xt = HCR_F32;
+    a.q = dst.as<int8_t>(); a.ldq = cols; a.scale = scale.as<float>();
+    a.rows = rows; a.cols = cols;
+    if (he == hipSuccess) rc = int8_rows_launch(I8_QUANT, a, st);
+    const hipError_t hs = hipStreamSynchronize(st);
+    if (rc == HCR_OK && (he != hipSuccess || hs != hipSuccess))
+      rc = hcr_set_errorf(HCR_EHIP, "int8 weights: %s", hipGetErrorString(he != hipSuccess ? he : hs));
+  }
+  tmp.release();
+  return rc;
+}
+
 static int upload_f32(DevBuf& dst, const float* src, size_t n, size_t n_pad, hipStream_t st) {
   CHECK(dst.ensure(n_pad * 4));
   HIPC(hipMemsetAsync(dst.p, 0, n_pad * 4, st));
@@ -230,7 +260,7 @@ static int upload_f32(DevBuf& dst, const float* src, size_t n, size_t n_pad, hip
   return HCR_OK;
 }
 
-template <typename TM, bool SPLIT>
+template <typename TM, bool SPLIT, bool I8 = false>
 static int finalize_t(hcr_encoder* e) {
   const auto& c = e->cfg;
   const int H = c.hidden, F = c.intermediate;
@@ -284,15 +314,22 @@ static int finalize_t(hcr_encoder* e) {
     std::memcpy(bqkv.data(), bq->data(), H * 4);
     std::memcpy(bqkv.data() + H, bk->data(), H * 4);
     std::memcpy(bqkv.data() + 2 * H, bv->data(), H * 4);
-    CHECK((upload_weights<TM, SPLIT>(L.wqkv, wqkv, 3 * H, H, rup(3 * H, 768), &L.sqkv, st)));
+    if constexpr (I8) {
+      CHECK(upload_weights_i8(L.wqkv, L.cqkv, wqkv, 3 * H, H, st));
+      CHECK(upload_weights_i8(L.wo, L.co, *wo, H, H, st));
+      CHECK(upload_weights_i8(L.wi, L.ci, *wi, F, H, st));
+      CHECK(upload_weights_i8(L.wo2, L.co2, *wo2, H, F, st));
+    } else {
+      CHECK((upload_weights<TM, SPLIT>(L.wqkv, wqkv, 3 * H, H, rup(3 * H, 768), &L.sqkv, st)));
+      CHECK((upload_weights<TM, SPLIT>(L.wo, *wo, H, H, rup(H, 768), &L.so, st)));
+      CHECK((upload_weights<TM, SPLIT>(L.wi, *wi, F, H, rup(F, 768), &L.si, st)));
+      CHECK((upload_weights<TM, SPLIT>(L.wo2, *wo2, H, F, rup(H, 768), &L.so2, st)));
+    }
     CHECK(upload_f32(L.bqkv, bqkv.data(), 3 * H, rup(3 * H, 768), st));
-    CHECK((upload_weights<TM, SPLIT>(L.wo, *wo, H, H, rup(H, 768), &L.so, st)));
     CHECK(upload_f32(L.bo, bo->data(), H, rup(H, 768), st));
     CHECK(upload_f32(L.ln1g, g1->data(), H, H, st));
     CHECK(upload_f32(L.ln1b, b1->data(), H, H, st));
-    CHECK((upload_weights<TM, SPLIT>(L.wi, *wi, F, H, rup(F, 768), &L.si, st)));
     CHECK(upload_f32(L.bi, bi->data(), F, rup(F, 768), st));
-    CHECK((upload_weights<TM, SPLIT>(L.wo2, *wo2, H, F, rup(H, 768), &L.so2, st)));
     CHECK(upload_f32(L.bo2, bo2->data(), H, rup(H, 768), st));
     CHECK(upload_f32(L.ln2g, g2->data(), H, H, st));
     CHECK(upload_f32(L.ln2b, b2->data(), H, H, st));
@@ -306,6 +343,7 @@ extern "C" int hcr_encoder_finalize(hcr_encoder* e) {
   HIPC(hipSetDevice(e->device));
   int rc = e->dtype == HCR_F16    ? finalize_t<_Float16, false>(e)
            : e->dtype == HCR_BF16 ? finalize_t<__bf16, false>(e)
+           : e->dtype == HCR_I8   ? finalize_t<_Float16, false, true>(e)
                                   : finalize_t<_Float16, true>(e);
   if (rc != HCR_OK) return rc;
   e->host.clear();
@@ -544,26 +582,25 @@ static int launch_attention_f32(hcr_encoder* e, EncWork& w, const int32_t* d_mas
   return HCR_OK;
 }
 
-template <typename TM, bool SPLIT>
-static int encode_t(hcr_encoder* e, EncWork& w, const int32_t* d_ids, const int32_t* d_mask, int64_t n, int S,
-                    float* d_out, hipStream_t st) {
-  const auto& c = e->cfg;
-  const int H = c.hidden, F = c.intermediate;
-  const int aw = SPLIT ? 3 : 1;                       // activation row width factor
-  int64_t T = n * (int64_t)S;
-  if (T > (int64_t)1 << 30) return hcr_set_error(HCR_EINVAL, "batch too large");
-  // Token packing (pack_tokens_kernel): only the tokens the result depends on run through the
-  // layers.  The packed row count is read back once (one stream synchronisation per batch):
-  // every grid below is sized by it.
+// The rows that run through the layers: T of them, packed (pack_tokens_kernel: only the tokens the
+// result depends on) with tok_map / seq_off set, or every position.  The packed row count is read
+// back once (one stream synchronisation per batch): every grid of the layers is sized by it.
+struct EncRows {
+  int64_t T = 0;
   const int32_t* tok_map = nullptr;
   const int32_t* seq_off = nullptr;
-  const int32_t* key_mask = d_mask;                   // per-row key bits: padded mask or packed
+  const int32_t* key_mask = nullptr;      // per-row key bits: padded mask or packed
+};
+static int pack_rows(hcr_encoder* e, EncWork& w, const int32_t* d_mask, int64_t n, int S, hipStream_t st, EncRows* r) {
+  int64_t T = n * (int64_t)S;
+  if (T > (int64_t)1 << 30) return hcr_set_error(HCR_EINVAL, "batch too large");
+  r->key_mask = d_mask;
   if (!enc_hooks().padded) {
     CHECK(w.pk_off.ensure((size_t)(n + 1) * 4));
     CHECK(w.pk_map.ensure((size_t)T * 4));
     CHECK(w.pk_ok.ensure((size_t)T * 4));
     CHECK(w.pk_tot.ensure(4));
-    hipLaunchKernelGGL(pack_tokens_kernel, dim3(1), dim3(1024), 0, st, d_mask, n, S, c.pooling == 1 ? 1 : 0,
+    hipLaunchKernelGGL(pack_tokens_kernel, dim3(1), dim3(1024), 0, st, d_mask, n, S, e->cfg.pooling == 1 ? 1 : 0,
                        w.pk_off.as<int32_t>(), w.pk_map.as<int32_t>(), w.pk_ok.as<int32_t>(),
                        w.pk_tot.as<int32_t>());
     HIPC(hipGetLastError());
@@ -571,10 +608,26 @@ static int encode_t(hcr_encoder* e, EncWork& w, const int32_t* d_ids, const int3
     HIPC(hipMemcpyAsync(&tot, w.pk_tot.p, 4, hipMemcpyDeviceToHost, st));
     HIPC(hipStreamSynchronize(st));
     T = tot;
-    tok_map = w.pk_map.as<const int32_t>();
-    seq_off = w.pk_off.as<const int32_t>();
-    key_mask = w.pk_ok.as<const int32_t>();
+    r->tok_map = w.pk_map.as<const int32_t>();
+    r->seq_off = w.pk_off.as<const int32_t>();
+    r->key_mask = w.pk_ok.as<const int32_t>();
   }
+  r->T = T;
+  return HCR_OK;
+}
+
+template <typename TM, bool SPLIT>
+static int encode_t(hcr_encoder* e, EncWork& w, const int32_t* d_ids, const int32_t* d_mask, int64_t n, int S,
+                    float* d_out, hipStream_t st) {
+  const auto& c = e->cfg;
+  const int H = c.hidden, F = c.intermediate;
+  const int aw = SPLIT ? 3 : 1;                       // activation row width factor
+  EncRows rows;
+  CHECK(pack_rows(e, w, d_mask, n, S, st, &rows));
+  const int64_t T = rows.T;
+  const int32_t* tok_map = rows.tok_map;
+  const int32_t* seq_off = rows.seq_off;
+  const int32_t* key_mask = rows.key_mask;
   if (T == 0) {                  // no token reaches the output (mean pooling, every mask 0)
     hipLaunchKernelGGL(pool_normalize_kernel, dim3((unsigned)n), dim3(256), 0, st, w.x.as<const float>(),
                        key_mask, seq_off, S, H, c.pooling, c.normalize, d_out);
@@ -678,6 +731,86 @@ static int encode_t(hcr_encoder* e, EncWork& w, const int32_t* d_ids, const int3
   return HCR_OK;
 }
 
+// HCR_I8: the layers on the int8 operators.  int8 rows (q8, s8) are what every product reads: the
+// LayerNorms leave those of x (their fp32 output, the residual stream), hcr_quant_rows' kernel those
+// of the attention's result and of the FFN activation.  Products leave f16; the residual is added in
+// fp32 by the LayerNorm that follows.
+static int encode_i8(hcr_encoder* e, EncWork& w, const int32_t* d_ids, const int32_t* d_mask, int64_t n, int S,
+                     float* d_out, hipStream_t st) {
+  const auto& c = e->cfg;
+  const int H = c.hidden, F = c.intermediate;
+  EncRows rows;
+  CHECK(pack_rows(e, w, d_mask, n, S, st, &rows));
+  const int64_t T = rows.T;
+  auto pool = [&]() -> int {
+    hipLaunchKernelGGL(pool_normalize_kernel, dim3((unsigned)n), dim3(256), 0, st, w.x.as<const float>(),
+                       rows.key_mask, rows.seq_off, S, H, c.pooling, c.normalize, d_out);
+    HIPC(hipGetLastError());
+    return HCR_OK;
+  };
+  if (T == 0) return pool();     // no token reaches the output (mean pooling, every mask 0)
+  CHECK(w.x.ensure((size_t)T * H * 4));
+  CHECK(w.y.ensure((size_t)T * H * 2));
+  CHECK(w.ctx.ensure((size_t)T * H * 2));
+  CHECK(w.qkv.ensure((size_t)T * 3 * H * 2));
+  CHECK(w.inter.ensure((size_t)T * F * 2));
+  CHECK(w.q8.ensure((size_t)T * std::max(H, F)));
+  CHECK(w.s8.ensure((size_t)T * 4));
+  // int8 rows of a [T][cols] buffer
+  auto quantise = [&](int mode, const DevBuf& x, int xt, int cols) -> int {
+    I8RowArgs a{};
+    a.x = x.p; a.ldx = cols; a.xt = xt;
+    a.q = w.q8.as<int8_t>(); a.ldq = cols; a.scale = w.s8.as<float>();
+    a.rows = T; a.cols = cols;
+    return int8_rows_launch(mode, a, st);
+  };
+  // x = LayerNorm(y + x), and its int8 rows
+  auto layer_norm = [&](const DevBuf& g, const DevBuf& b) -> int {
+    I8RowArgs a{};
+    a.x = w.y.p; a.ldx = H; a.xt = HCR_F16;
+    a.r = w.x.p; a.ldr = H; a.rt = HCR_F32;
+    a.y = w.x.p; a.ldy = H; a.yt = HCR_F32;
+    a.g = g.as<const float>(); a.b = b.as<const float>(); a.eps = c.layer_norm_eps;
+    a.q = w.q8.as<int8_t>(); a.ldq = H; a.scale = w.s8.as<float>();
+    a.rows = T; a.cols = H;
+    return int8_rows_launch(I8_LAYER, a, st);
+  };
+  auto linear = [&](const DevBuf& wt, const DevBuf& ws, const DevBuf& bias, int K, int N, const DevBuf& out) -> int {
+    I8LinearArgs a{};
+    a.x = w.q8.as<const int8_t>(); a.ldx = K; a.sx = w.s8.as<const float>();
+    a.w = wt.as<const int8_t>(); a.ldw = K; a.sw = ws.as<const float>();
+    a.bias = bias.as<const float>(); a.out = out.p; a.ldo = N; a.ot = HCR_F16;
+    a.T = (int)T; a.N = N; a.K = K; a.vec = 1;
+    return int8_linear_launch(a, st);
+  };
+  const unsigned gT = (unsigned)((T + 3) / 4);
+  // (the f16 copy that the embedding kernels leave is not used here: it lands in y)
+  if (H <= 1024 && !enc_hooks().ln_scalar)
+    hipLaunchKernelGGL((embed_ln4_kernel<_Float16, false>), dim3(gT), dim3(256), 0, st, d_ids, rows.tok_map, (int)T, S,
+                       H, e->wemb.as<const float>(), e->pemb.as<const float>(), e->temb.as<const float>(),
+                       e->embg.as<const float>(), e->embb.as<const float>(), c.layer_norm_eps, w.x.as<float>(),
+                       w.y.as<_Float16>());
+  else
+    hipLaunchKernelGGL((embed_ln_kernel<_Float16, false>), dim3(gT), dim3(256), 0, st, d_ids, rows.tok_map, (int)T, S,
+                       H, e->wemb.as<const float>(), e->pemb.as<const float>(), e->temb.as<const float>(),
+                       e->embg.as<const float>(), e->embb.as<const float>(), c.layer_norm_eps, w.x.as<float>(),
+                       w.y.as<_Float16>());
+  HIPC(hipGetLastError());
+  CHECK(quantise(I8_QUANT, w.x, HCR_F32, H));
+  for (const EncLayer& L : e->layers) {
+    CHECK(linear(L.wqkv, L.cqkv, L.bqkv, H, 3 * H, w.qkv));
+    CHECK(launch_attention<_Float16>(e, w, rows.key_mask, rows.seq_off, n, S, st));
+    CHECK(quantise(I8_QUANT, w.ctx, HCR_F16, H));
+    CHECK(linear(L.wo, L.co, L.bo, H, H, w.y));
+    CHECK(layer_norm(L.ln1g, L.ln1b));
+    CHECK(linear(L.wi, L.ci, L.bi, H, F, w.inter));
+    CHECK(quantise(I8_GELU, w.inter, HCR_F16, F));
+    CHECK(linear(L.wo2, L.co2, L.bo2, F, H, w.y));
+    CHECK(layer_norm(L.ln2g, L.ln2b));
+  }
+  return pool();
+}
+
 extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int32_t* d_mask,
                                  int64_t n, int S, float* d_out, void* stream) {
   if (!e) return hcr_set_error(HCR_EINVAL, "encoder is NULL");
@@ -694,6 +827,7 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
     float* out = d_out + s0 * e->cfg.hidden;
     if (e->dtype == HCR_F16) return encode_t<_Float16, false>(e, w, ids, mask, ns, S, out, ws);
     if (e->dtype == HCR_BF16) return encode_t<__bf16, false>(e, w, ids, mask, ns, S, out, ws);
+    if (e->dtype == HCR_I8) return encode_i8(e, w, ids, mask, ns, S, out, ws);
     return encode_t<_Float16, true>(e, w, ids, mask, ns, S, out, ws);
   };
   // r04a A/B (bge-base, 1024 x S = 32 ragged, one box): f16 142.3k -> 149.7-152.0k embeddings/s

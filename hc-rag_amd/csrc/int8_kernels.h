@@ -6,6 +6,7 @@
 #pragma once
 #include "device_common.h"
 #include "hcrag.h"
+#include "int8_args.h"
 
 namespace hcr {
 
@@ -26,22 +27,6 @@ typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 // finite value, and such a row gets scale NaN and q = 0, so that a product with it is NaN.  A row
 // below 2^-100 counts as zeros (scale 0, q 0): 127 / a would leave fp32's range.
 // -------------------------------------------------------------------------------------
-enum : int { I8_QUANT = 0, I8_GELU = 1, I8_LAYER = 2, I8_RMS = 3 };
-
-struct I8RowArgs {
-  const void* x; int64_t ldx;
-  const void* r; int64_t ldr;      // residual (NULL: none)
-  void* sum; int64_t ldsum;        // h in r's type (NULL: not stored); may be r itself
-  void* y; int64_t ldy;            // v in yt (NULL: not stored); may be x or r itself
-  const float* g; const float* b;  // (b NULL: 0)
-  int8_t* q; int64_t ldq;
-  float* scale;
-  int64_t rows;
-  int cols;
-  float eps;
-  int xt, rt, yt;                  // hcr_dtype of x, r (and sum), y
-};
-
 // gelu(x) = x Phi(x) = x / (1 + 2^-z), z = log2(Phi / (1 - Phi)) = x g(x^2): g as a polynomial fitted so
 // that Phi is within 2.9e-8 everywhere (its last coefficient is positive: z keeps x's sign past the
 // fit, where Phi is 0 or 1).  7 instructions fewer per element than erf_as's form, whose division
@@ -116,10 +101,14 @@ __device__ __forceinline__ void i8_convert(float (&v)[8], const I8Raw& o, int ty
     }
   }
 }
+// Both rounded at once (v_cvt_pk): element by element, the f16 conversion after an fma becomes one
+// v_fma_mixlo, which leaves f16 subnormals as zeros.
 template <typename T>
-__device__ __forceinline__ uint32_t i8_bits16(float v) { return __builtin_bit_cast(uint16_t, (T)v); }
-template <typename T>
-__device__ __forceinline__ uint32_t i8_pack2(float x, float y) { return i8_bits16<T>(x) | i8_bits16<T>(y) << 16; }
+__device__ __forceinline__ uint32_t i8_pack2(float x, float y) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{x, y}), T2));
+}
 // elements [i, i + 8) of a row of cols, those that exist
 __device__ __forceinline__ void i8_store(char* row, int type, int i, int cols, const float (&v)[8]) {
   if (type == HCR_F32) {
@@ -379,15 +368,6 @@ int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __re
 // K need not fill a stage: w's bytes at k >= K are replaced by zeros in registers, so what the
 // padding of either operand holds does not matter.
 // -------------------------------------------------------------------------------------
-struct I8LinearArgs {
-  const int8_t* x; int64_t ldx; const float* sx;
-  const int8_t* w; int64_t ldw; const float* sw;
-  const float* bias;               // (NULL: 0)
-  void* out; int64_t ldo; int ot;  // hcr_dtype of out
-  int T, N, K;
-  int vec;                         // out's rows start on 4 elements
-};
-
 __device__ __forceinline__ intx4 i8_mfma(intx4 a, intx4 b, intx4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
@@ -412,14 +392,13 @@ __device__ __forceinline__ void i8_store_out4(const I8LinearArgs& a, int64_t t, 
       for (int r = 0; r < 4; ++r) if (f + r < a.N) p[r] = v[r];
     return;
   }
-  uint32_t h[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) h[r] = a.ot == HCR_BF16 ? i8_bits16<__bf16>(v[r]) : i8_bits16<_Float16>(v[r]);
+  const uint2 h = a.ot == HCR_BF16 ? uint2{i8_pack2<__bf16>(v[0], v[1]), i8_pack2<__bf16>(v[2], v[3])}
+                                   : uint2{i8_pack2<_Float16>(v[0], v[1]), i8_pack2<_Float16>(v[2], v[3])};
   uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + t * a.ldo + f;
-  if (a.vec && f + 4 <= a.N) *reinterpret_cast<uint2*>(p) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+  if (a.vec && f + 4 <= a.N) *reinterpret_cast<uint2*>(p) = h;
   else
 #pragma unroll
-    for (int r = 0; r < 4; ++r) if (f + r < a.N) p[r] = (uint16_t)h[r];
+    for (int r = 0; r < 4; ++r) if (f + r < a.N) p[r] = (uint16_t)((r < 2 ? h.x : h.y) >> (16 * (r & 1)));
 }
 
 // Operands straight from memory to the matrix cores: 16 features x 16 TB tokens per workgroup,

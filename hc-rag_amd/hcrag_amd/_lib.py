@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get(
     "HCRAG_LIB", os.path.join(os.path.dirname(_HERE), "lib", "libhcrag_hip.so"))
 
 HCR_OK, HCR_EINVAL, HCR_EHIP, HCR_ERCCL, HCR_ENOMEM, HCR_EIO, HCR_EINTERNAL = 0, -1, -2, -3, -4, -5, -6
-HCR_F16, HCR_BF16, HCR_F32 = 0, 1, 2
+HCR_F16, HCR_BF16, HCR_F32, HCR_I8 = 0, 1, 2, 3
 HCR_SCORE_COSINE, HCR_SCORE_UNIT = 0, 1
 HCR_ACT_NONE, HCR_ACT_GELU = 0, 1
 HCR_NORM_LAYER, HCR_NORM_RMS = 0, 1

@@ -29,13 +29,15 @@ import numpy as np
 from ._lib import BertConfig, check, lib
 from .tokenizer import WordPieceTokenizer
 
-HCR_F16, HCR_BF16, HCR_F32 = 0, 1, 2
+HCR_F16, HCR_BF16, HCR_F32, HCR_I8 = 0, 1, 2, 3
 # "f32": reference precision (split-f16 MFMA GEMMs, fp32 attention / LayerNorm; the reference
 # encodes in fp32 torch, experiments/embedding_generator.py:124) -- the default.
 # "f16" / "bf16": fast modes (16-bit MFMA operands, fp32 accumulation).
+# "i8": fastest (projections as 8-bit integer products with scales per token and channel; the
+# embeddings are the quantised model's).
 _DTYPES = {"f32": HCR_F32, "fp32": HCR_F32, "float32": HCR_F32,
            "f16": HCR_F16, "fp16": HCR_F16, "float16": HCR_F16,
-           "bf16": HCR_BF16, "bfloat16": HCR_BF16}
+           "bf16": HCR_BF16, "bfloat16": HCR_BF16, "i8": HCR_I8, "int8": HCR_I8}
 
 # all-MiniLM-L6-v2 (the reference's model, experiments/embedding_generator.py:21)
 MINILM_L6_V2 = dict(vocab_size=30522, hidden=384, layers=6, heads=12, intermediate=1536,
@@ -68,7 +70,7 @@ class BertEncoder:
 
     def __init__(self, config: Mapping, state_dict: Mapping, dtype: str = "f32", device: int = 0):
         if dtype not in _DTYPES:
-            raise ValueError(f"unknown encoder dtype {dtype!r} (f32 | f16 | bf16)")
+            raise ValueError(f"unknown encoder dtype {dtype!r} (f32 | f16 | bf16 | i8)")
         self.config = dict(config)
         self.hidden = int(self.config["hidden"])
         self.max_position = int(self.config["max_position"])

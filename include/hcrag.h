@@ -37,7 +37,8 @@ typedef enum {
                         outside the index): the call is abandoned, the handle stays usable */
 } hcr_status;
 
-typedef enum { HCR_F16 = 0, HCR_BF16 = 1, HCR_F32 = 2 } hcr_dtype;
+/* (HCR_I8: a compute mode of the encoder only, not a storage or buffer type) */
+typedef enum { HCR_F16 = 0, HCR_BF16 = 1, HCR_F32 = 2, HCR_I8 = 3 } hcr_dtype;
 
 /* What hcr_quant_rows_device applies to a value before it is quantised (GELU: exact-erf form). */
 typedef enum { HCR_ACT_NONE = 0, HCR_ACT_GELU = 1 } hcr_activation;
@@ -316,7 +317,12 @@ typedef struct hcr_encoder hcr_encoder;
  *            are deterministic for a given batch but may differ by fp32 rounding (<= 1e-5)
  *            between batches that contain it (torch's own GEMMs are batch-dependent likewise);
  *   HCR_F16 / HCR_BF16  fast: f16 / bf16 MFMA operands (accumulation, LayerNorm, softmax and
- *            the residual stream fp32). */
+ *            the residual stream fp32);
+ *   HCR_I8   fastest: the projections as 8-bit integer products (weights with a scale per output
+ *            channel, activations with a scale per token, quantised as the int8 operators below
+ *            do), f16 attention and product outputs, fp32 LayerNorm, GELU and residual stream.
+ *            Quantisation is part of the result: cosine to fp32 BertModel about 0.999, not the
+ *            16-bit modes' 0.9999.  Needs intermediate <= 32768. */
 int hcr_encoder_create(int device, const hcr_bert_config* cfg, int compute_dtype,
                        hcr_encoder** out);
 int hcr_encoder_compute_dtype(const hcr_encoder* enc);

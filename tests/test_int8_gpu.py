@@ -109,6 +109,34 @@ def test_linear_strides_and_what_lies_around(T, N, K, out):
 
 
 @gpu
+@pytest.mark.parametrize("T", [3, 100, 1000, 9000, 66000])
+def test_linear_f16_subnormal_results(T):
+    """Results below f16's normal range keep its subnormal steps (bound: half of one)."""
+    m, g = _ops(), _gen(T)
+    for N, K in ((257, 96), (1024, 1024)):
+        x, w = _int8(g, T, K), _int8(g, N, K)
+        sx, sw = _scales(g, T) * 2.0 ** -10, _scales(g, N) * 2.0 ** -14
+        y = m.int8_linear(m.Int8Rows(x, sx), m.Int8Rows(w, sw), dtype=torch.float16)
+        assert bool((y[:, :64].abs() < 6e-5).any()) and bool((y != 0).any())
+        _linear_check(y, x, sx, w, sw, None)
+
+
+@gpu
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+def test_linear_rows_do_not_depend_on_the_batch(out):
+    """The same row through every kernel and chunk: the same bits."""
+    m, g = _ops(), _gen(17)
+    for N, K in ((384, 384), (1155, 1100), (4096, 1024)):
+        T = 20000
+        x, w, sx, sw = _int8(g, T, K), _int8(g, N, K), _scales(g, T), _scales(g, N)
+        bias = torch.randn(N, generator=g, device="cuda")
+        W = m.Int8Rows(w, sw)
+        y = m.int8_linear(m.Int8Rows(x, sx), W, bias=bias, dtype=DT[out])
+        for n in (1, 16, 40, 200, 700, 3000, 9000):
+            assert torch.equal(m.int8_linear(m.Int8Rows(x[:n], sx[:n]), W, bias=bias, dtype=DT[out]), y[:n])
+
+
+@gpu
 def test_linear_offsets_past_32_bits():
     m, g = _ops(), _gen(3)
     T, N, K = (1 << 17) + 3, 16400, 17
