@@ -83,12 +83,14 @@ __host__ __device__ constexpr int i8_size(int ot) { return ot == HCR_F32 ? 4 : 2
 // quads are exchanged between neighbouring 16-lane rows, after which a lane holds 8 features of a
 // token and a store covers 16 tokens x 64 bytes (f32: 4 features, the same 64 bytes).  The 2 MT
 // (f32: 4 MT) 16-byte buffer stores are unconditional -- what lies outside is dropped by the
-// descriptor -- so that a wave issues that many for every tile; features of a row's last, partial
-// 16 bytes follow one by one.  (Rows need only their elements' alignment.)
+// descriptor -- so that a wave issues that many for every tile; with ODD (a row is no
+// whole number of 16 bytes) the features of its last, partial 16 bytes follow one by one.  (Rows need
+// only their elements' alignment.)  Without the ODD code the stream kernel holds 30 registers less:
+// T = 21853, N = 2304, K = 768 57 us, with it 64.
 // sw, sb, sx: LDS addresses of the wave's w scales, biases and x scales.
 // Measured against staging the tile through LDS for 256-byte stores, with 128 x 256 tiles of 4 waves
 // at K = 768, N = 2304, T = 21853: 60.8 us, staged 62.8.
-template <int OT, int MT>
+template <int OT, int MT, bool ODD>
 __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_buffer_rsrc_t o_rsrc,
                                               const intx4 (&acc)[MT][4], int lane, int f0, int t0, uint32_t sw,
                                               uint32_t sb, uint32_t sx) {
@@ -143,7 +145,7 @@ __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_bu
 #pragma unroll
       for (int j = 0; j < NU; ++j) {
         __builtin_amdgcn_raw_buffer_store_b128(u[j], o_rsrc, f[j] + PER <= left ? row[n] + f[j] * ES : I8_FAR, 0, 0);
-        if (left < 16 * MT && left % PER) {            // (uniform: the wave's last features, odd widths)
+        if (ODD && left < 16 * MT) {                   // (uniform: the wave holds the row's last features)
           const uint32_t w[4] = {u[j][0], u[j][1], u[j][2], u[j][3]};
 #pragma unroll
           for (int e = 0; e < PER - 1; ++e) {
@@ -158,7 +160,7 @@ __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_bu
 }
 
 // A workgroup of WM x WN waves per tile of 16 MT WM features x 64 WN tokens; OCC waves per SIMD.
-template <int OT, int MT, int WM, int WN, int NST, int OCC>
+template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC>
 __global__ void __launch_bounds__(64 * WM * WN, OCC)
 int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
   constexpr int KB = 64, FT = 16 * MT * WM, TT = 64 * WN, NW = WM * WN;
@@ -191,22 +193,24 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
       uniform_ptr(a.x), (short)0, (a.T - 1) * (int)a.ldx + kend, 0x00020000);
   const int drow = lane >> 2;
   const int dchunk = (lane & 3) ^ (int)((V3_SWZ >> (((lane >> 4) & 3) * 4)) & 3u);
-  const int voff_w = (f0 + drow) * (int)a.ldw + dchunk * 16, voff_x = (t0 + drow) * (int)a.ldx + dchunk * 16;
+  // A piece's offset of rows is in the lane's part, only the depth (below the operand's size) in the
+  // scalar part: a range check compares the first with the size less the second.
+  int voff[NPC];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) voff[i] = (f0 + (wave + NW * i) * 16 + drow) * (int)a.ldw + dchunk * 16;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) voff[NA + i] = (t0 + (wave + NW * i) * 16 + drow) * (int)a.ldx + dchunk * 16;
   const int nsteps = (a.K + KB - 1) / KB;
   int is_s = 0, is_slot = 0;
   auto issue = [&](auto piece) __attribute__((always_inline)) {
     constexpr int i = decltype(piece)::value;
     // (past the last stage the pieces are still issued, for the waits' counts, but read nothing)
-    const int far = __builtin_amdgcn_readfirstlane(is_s < nsteps ? 0 : I8_FAR);
-    const int kofs = __builtin_amdgcn_readfirstlane(is_s * KB);
+    const bool live = is_s < nsteps;
+    const int far = __builtin_amdgcn_readfirstlane(live ? 0 : I8_FAR);
+    const int kofs = __builtin_amdgcn_readfirstlane(live ? is_s * KB : 0);
     char* st = ring + __builtin_amdgcn_readfirstlane(is_slot) * STAGE;
-    if constexpr (i < NA) {
-      const int j = wave + NW * i;
-      dma16(w_rsrc, st + j * 1024, voff_w | far, __builtin_amdgcn_readfirstlane(j * 16 * (int)a.ldw + kofs));
-    } else {
-      const int j = wave + NW * (i - NA);
-      dma16(x_rsrc, st + A_BYTES + j * 1024, voff_x | far, __builtin_amdgcn_readfirstlane(j * 16 * (int)a.ldx + kofs));
-    }
+    if constexpr (i < NA) dma16(w_rsrc, st + (wave + NW * i) * 1024, voff[i] | far, kofs);
+    else dma16(x_rsrc, st + A_BYTES + (wave + NW * (i - NA)) * 1024, voff[i] | far, kofs);
   };
   auto advance = [&]() __attribute__((always_inline)) {
     ++is_s;
@@ -250,11 +254,11 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
     advance();
     rslot = (rslot + 1 == NST) ? 0 : rslot + 1;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the ring's last pieces, before the LDS is given back
   const __amdgpu_buffer_rsrc_t o_rsrc = __builtin_amdgcn_make_buffer_rsrc(
       uniform_ptr(a.out), (short)0, __builtin_amdgcn_readfirstlane(((a.T - 1) * (int)a.ldo + a.N) * i8_size(OT)), 0x00020000);
-  i8_store_tile<OT, MT>(a, o_rsrc, acc, lane, f0 + wm * 16 * MT, t0 + wn * 64, lds_addr(sc + wm * 16 * MT),
+  i8_store_tile<OT, MT, ODD>(a, o_rsrc, acc, lane, f0 + wm * 16 * MT, t0 + wn * 64, lds_addr(sc + wm * 16 * MT),
                         lds_addr(sc + FT + wm * 16 * MT), lds_addr(sc + 2 * FT + wn * 64));
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the ring's last pieces, before the LDS is given back
 }
 
 // -------------------------------------------------------------------------------------
@@ -275,7 +279,7 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
 //     4 stages ahead of group 1's epilogue: at 2 stages a tile, 2 tiles).
 // Host-checked: K > 64 (2 stages a tile at least).
 // OT: hcr_dtype of out
-template <int OT>
+template <int OT, bool ODD>
 __global__ void __launch_bounds__(512, 2)
 int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
   constexpr int KB = 64, NST = 4, FT = 256, TT = 256, A_BYTES = FT * KB, STAGE = (FT + TT) * KB;
@@ -310,7 +314,6 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
 
   const int drow = lane >> 2;
   const int dchunk = (lane & 3) ^ (int)((V3_SWZ >> (((lane >> 4) & 3) * 4)) & 3u);
-  const int voff_w = drow * (int)a.ldw + dchunk * 16, voff_x = drow * (int)a.ldx + dchunk * 16;
   const int nsteps = (a.K + KB - 1) / KB;
   auto tile_at = [&](int i, int& f0, int& t0) __attribute__((always_inline)) {
     const unsigned g = first + mine + (unsigned)i * per;
@@ -318,7 +321,8 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
     t0 = __builtin_amdgcn_readfirstlane((int)(g / (unsigned)n_tiles_feat) * TT);
   };
   // the stream's head: stage is_s of tile is_i, bound for slot is_slot
-  int is_s = 0, is_i = 0, is_slot = 0, is_w = 0, is_x = 0;
+  int is_s = 0, is_i = 0, is_slot = 0;
+  int voff[4];                                         // (rows here, the depth in the scalar part: see above)
   auto issue_stage = [&]() __attribute__((always_inline)) {
     const bool live = is_i < my_tiles;
     // (past the last tile the pieces are still issued, for the waits' counts, but read nothing)
@@ -326,24 +330,22 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
     if (live && is_s == 0) {
       int f0, t0;
       tile_at(is_i, f0, t0);
-      is_w = f0 * (int)a.ldw;
-      is_x = t0 * (int)a.ldx;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = (wave + 8 * i) * 16 + drow;
+        voff[i] = (f0 + r) * (int)a.ldw + dchunk * 16;
+        voff[2 + i] = (t0 + r) * (int)a.ldx + dchunk * 16;
+      }
       char* s = reinterpret_cast<char*>(sc[is_i & 3]);
-      dma4(f_rsrc, s + wave * 256, lane * 4, (f0 + (wave & 3) * 64) * 4);
-      if (wave < 4) dma4(sx_rsrc, s + 2 * FT * 4 + wave * 256, lane * 4, (t0 + wave * 64) * 4);
+      dma4(f_rsrc, s + wave * 256, (f0 + (wave & 3) * 64 + lane) * 4, 0);
+      if (wave < 4) dma4(sx_rsrc, s + 2 * FT * 4 + wave * 256, (t0 + wave * 64 + lane) * 4, 0);
     }
-    const int kofs = is_s * KB;
+    const int kofs = __builtin_amdgcn_readfirstlane(live ? is_s * KB : 0);
     char* st = ring + __builtin_amdgcn_readfirstlane(is_slot) * STAGE;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = wave + 8 * i;
-      dma16(w_rsrc, st + j * 1024, voff_w | far, __builtin_amdgcn_readfirstlane(is_w + j * 16 * (int)a.ldw + kofs));
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = wave + 8 * i;
-      dma16(x_rsrc, st + A_BYTES + j * 1024, voff_x | far, __builtin_amdgcn_readfirstlane(is_x + j * 16 * (int)a.ldx + kofs));
-    }
+    dma16(w_rsrc, st + wave * 1024, voff[0] | far, kofs);
+    dma16(w_rsrc, st + (wave + 8) * 1024, voff[1] | far, kofs);
+    dma16(x_rsrc, st + A_BYTES + wave * 1024, voff[2] | far, kofs);
+    dma16(x_rsrc, st + A_BYTES + (wave + 8) * 1024, voff[3] | far, kofs);
     is_slot = (is_slot + 1) & (NST - 1);
     if (++is_s == nsteps) { is_s = 0; ++is_i; }
   };
@@ -363,7 +365,7 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
     int f0, t0;
     tile_at(i, f0, t0);
     const uint32_t s0 = lds_addr(sc[i & 3]);
-    i8_store_tile<OT, 8>(a, o_rsrc, acc, lane, f0 + wm * 128, t0 + wn * 64, s0 + wm * 512, s0 + (FT + wm * 128) * 4,
+    i8_store_tile<OT, 8, ODD>(a, o_rsrc, acc, lane, f0 + wm * 128, t0 + wn * 64, s0 + wm * 512, s0 + (FT + wm * 128) * 4,
                          s0 + (2 * FT + wn * 64) * 4);
   };
 
@@ -376,10 +378,12 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
   for (int ti = 0; ti < my_tiles; ++ti) {
     for (int s = 0; s < nsteps; ++s) {
       issue_stage();
+      __builtin_amdgcn_sched_barrier(0);               // the stores stay behind these pieces (the waits' counts)
       if (s == 0 && ti) {
         store_tile(ti - 1);
         clear();
       }
+      __builtin_amdgcn_sched_barrier(0);
       const char* st = ring + rslot * STAGE;
       intx4 av[8], bq[4];
       i8_read_frags(lds_addr(st + offA), lds_addr(st + offB), av, bq);
@@ -405,8 +409,8 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
     }
   }
   if (!grp) v3_barrier();
-  store_tile(my_tiles - 1);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the ring's last pieces, before the LDS is given back
+  store_tile(my_tiles - 1);
 }
 
 }  // namespace hcr

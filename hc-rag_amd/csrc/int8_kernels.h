@@ -401,56 +401,74 @@ __device__ __forceinline__ void i8_store_out4(const I8LinearArgs& a, int64_t t, 
     for (int r = 0; r < 4; ++r) if (f + r < a.N) p[r] = (uint16_t)((r < 2 ? h.x : h.y) >> (16 * (r & 1)));
 }
 
-// Operands straight from memory to the matrix cores: 16 features x 16 TB tokens per workgroup,
+// Operands straight from memory to the matrix cores: 16 FB features x 16 TB tokens per workgroup,
 // whose KW waves take every KW-th 128-byte piece of the rows (a lane's 32 bytes are contiguous,
 // a row's 128 bytes one line; the contraction order is the same for both operands) and add their
 // int32 sums through LDS.
-template <int TB, int KW>
+template <int FB, int TB, int KW>
 __global__ void __launch_bounds__(64 * KW)
 int8_linear_direct(I8LinearArgs a) {
-  __shared__ __attribute__((aligned(16))) intx4 red[KW][TB][64];
+  __shared__ __attribute__((aligned(16))) intx4 red[KW][FB * TB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int li = lane & 15, lg = lane >> 4;
-  const unsigned nfb = (unsigned)((a.N + 15) >> 4);
-  const int f0 = (int)(blockIdx.x % nfb) * 16, t0 = (int)(blockIdx.x / nfb) * (16 * TB);
-  const int8_t* wr = a.w + (int64_t)min(f0 + li, a.N - 1) * a.ldw;
+  const unsigned nfb = (unsigned)((a.N + 16 * FB - 1) / (16 * FB));
+  const int f0 = (int)(blockIdx.x % nfb) * (16 * FB), t0 = (int)(blockIdx.x / nfb) * (16 * TB);
+  const int8_t* wr[FB];
   const int8_t* xr[TB];
 #pragma unroll
-  for (int b = 0; b < TB; ++b) xr[b] = a.x + (int64_t)min(t0 + 16 * b + li, a.T - 1) * a.ldx;
-  intx4 acc[TB];
+  for (int c = 0; c < FB; ++c) wr[c] = a.w + (int64_t)min(f0 + 16 * c + li, a.N - 1) * a.ldw;
 #pragma unroll
-  for (int b = 0; b < TB; ++b) acc[b] = intx4{0, 0, 0, 0};
+  for (int b = 0; b < TB; ++b) xr[b] = a.x + (int64_t)min(t0 + 16 * b + li, a.T - 1) * a.ldx;
+  intx4 acc[FB][TB];
+#pragma unroll
+  for (int c = 0; c < FB; ++c)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[c][b] = intx4{0, 0, 0, 0};
   const int whole = a.K / 128 * 128;
   for (int k = wave * 128; k < whole; k += KW * 128) {
-    const intx4* wp = reinterpret_cast<const intx4*>(wr + k + lg * 32);
-    const intx4 w0 = wp[0], w1 = wp[1];
+    intx4 w[FB][2], x[TB][2];
 #pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      const intx4* xp = reinterpret_cast<const intx4*>(xr[b] + k + lg * 32);
-      acc[b] = i8_mfma(w0, xp[0], acc[b]);
-      acc[b] = i8_mfma(w1, xp[1], acc[b]);
-    }
+    for (int c = 0; c < FB; ++c)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) w[c][j] = reinterpret_cast<const intx4*>(wr[c] + k + lg * 32)[j];
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[b][j] = reinterpret_cast<const intx4*>(xr[b] + k + lg * 32)[j];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < FB; ++c)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) acc[c][b] = i8_mfma(w[c][j], x[b][j], acc[c][b]);
   }
   if (whole < a.K && (whole / 128) % KW == wave) {      // the rows' last, partial piece
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int k = whole + lg * 32 + j * 16, n = a.K - k;
       const int kk = n > 0 ? k : 0;                     // (a chunk past the row: any, times 0)
-      const intx4 w0 = i8_keep(*reinterpret_cast<const intx4*>(wr + kk), n);
+      intx4 x[TB];
 #pragma unroll
-      for (int b = 0; b < TB; ++b)
-        acc[b] = i8_mfma(w0, *reinterpret_cast<const intx4*>(xr[b] + kk), acc[b]);
+      for (int b = 0; b < TB; ++b) x[b] = *reinterpret_cast<const intx4*>(xr[b] + kk);
+#pragma unroll
+      for (int c = 0; c < FB; ++c) {
+        const intx4 w = i8_keep(*reinterpret_cast<const intx4*>(wr[c] + kk), n);
+#pragma unroll
+        for (int b = 0; b < TB; ++b) acc[c][b] = i8_mfma(w, x[b], acc[c][b]);
+      }
     }
   }
 #pragma unroll
-  for (int b = 0; b < TB; ++b) red[wave][b][lane] = acc[b];
-  __syncthreads();
-  for (int b = wave; b < TB; b += KW) {
-    intx4 s = red[0][b][lane];
+  for (int c = 0; c < FB; ++c)
 #pragma unroll
-    for (int w = 1; w < KW; ++w) s += red[w][b][lane];
-    // lane: features f0 + 4 lg .. + 3 of token t0 + 16 b + li
-    const int t = t0 + 16 * b + li, f = f0 + 4 * lg;
+    for (int b = 0; b < TB; ++b) red[wave][c * TB + b][lane] = acc[c][b];
+  __syncthreads();
+  for (int i = wave; i < FB * TB; i += KW) {
+    intx4 s = red[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) s += red[w][i][lane];
+    // lane: features f .. f + 3 of token t
+    const int t = t0 + 16 * (i % TB) + li, f = f0 + 16 * (i / TB) + 4 * lg;
     if (t >= a.T || f >= a.N) continue;
     const float sx = a.sx[t];
     float v[4];

@@ -42,52 +42,65 @@ int int8_rows_launch(int mode, const I8RowArgs& a, hipStream_t st) {
   return HCR_OK;
 }
 
-template <int TB, int KW>
+template <int FB, int TB, int KW>
 static int launch_direct(const I8LinearArgs& a, hipStream_t st) {
-  const int64_t blocks = (int64_t)((a.N + 15) / 16) * ((a.T + 16 * TB - 1) / (16 * TB));
+  const int64_t blocks = (int64_t)((a.N + 16 * FB - 1) / (16 * FB)) * ((a.T + 16 * TB - 1) / (16 * TB));
   if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many outputs for one call");
-  hipLaunchKernelGGL((int8_linear_direct<TB, KW>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
+  hipLaunchKernelGGL((int8_linear_direct<FB, TB, KW>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
   HIPC(hipGetLastError());
   return HCR_OK;
 }
 // 128 features x 256 tokens per workgroup of 8 waves (64 x 64 each), two workgroups per CU
-template <int OT>
+template <int OT, bool ODD>
 static void launch_tiles(const I8LinearArgs& a, hipStream_t st) {
   const int nft = (a.N + 127) / 128;
   const int tiles = nft * ((a.T + 255) / 256);
-  hipLaunchKernelGGL((int8_linear_tiles<OT, 4, 2, 4, 3, 4>), dim3((unsigned)tiles), dim3(512), 0, st, a, nft);
+  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD, 4, 2, 4, 3, 4>), dim3((unsigned)tiles), dim3(512), 0, st, a, nft);
 }
-template <int OT>
+template <int OT, bool ODD>
 static void launch_stream(const I8LinearArgs& a, hipStream_t st) {
   const int nft = (a.N + 255) / 256;
   const unsigned tiles = (unsigned)nft * ((a.T + 255) / 256);
-  hipLaunchKernelGGL((int8_linear_stream<OT>), dim3(std::min((tiles + 7) & ~7u, 256u)), dim3(512), 0, st, a, nft, tiles);
+  hipLaunchKernelGGL((int8_linear_stream<OT, ODD>), dim3(std::min((tiles + 7) & ~7u, 256u)), dim3(512), 0, st, a, nft, tiles);
 }
 template <int OT>
 static void launch_linear(const I8LinearArgs& a, bool stream, hipStream_t st) {
-  if (stream) launch_stream<OT>(a, st);
-  else launch_tiles<OT>(a, st);
+  const bool odd = a.N % (16 / i8_size(OT)) != 0;
+  if (stream) odd ? launch_stream<OT, true>(a, st) : launch_stream<OT, false>(a, st);
+  else odd ? launch_tiles<OT, true>(a, st) : launch_tiles<OT, false>(a, st);
 }
 
-// Which kernel (MI355X, us, tiles of 128 x 256 / 256 x 256 counted over the whole output):
-//   direct  below 32 tiles of 128 x 256, the workgroup's tokens as wide as leaves 256 workgroups
-//           (K = 4096, N = 1024: T = 512 20.5, tiles 31; T = 1024 38, tiles 31; K = 1024, N = 4096:
-//           T = 256 12.0, tiles 10.9; T = 512 21.6, tiles 11)
+// Features and tokens per workgroup of the direct kernel, in 16s: the wider the less it reads for an
+// output, as long as the device is filled (us on MI355X; G the number of workgroups):
+//   2 x 4  from 256 of them at depths where reading dominates (T = 512, N = 1024, K = 4096: 14.4, with
+//          2 x 2 17.3; K = 384, N = 1152: 5.4, 4.9)
+//   2 x 2  from 144 (T = 256, N = 768, K = 768: 4.0, with 1 x 2 4.5; T = 128, G = 96: 3.9, 3.5)
+//   1 x 2  from 192 (T = 128, N = 1024, K = 4096: 8.0, with 1 x 1 9.6; T = 64, G = 128: 7.8, 5.9)
+static int launch_direct_for(const I8LinearArgs& a, hipStream_t st) {
+  auto groups = [&](int fb, int tb) { return (int64_t)((a.N + 16 * fb - 1) / (16 * fb)) * ((a.T + 16 * tb - 1) / (16 * tb)); };
+  if (a.T > 16) {
+    if (a.K >= 1024 && groups(2, 4) >= 256) return launch_direct<2, 4, 4>(a, st);
+    if (groups(2, 2) >= 144) return launch_direct<2, 2, 4>(a, st);
+    if (groups(1, 2) >= 192) return launch_direct<1, 2, 4>(a, st);
+  }
+  return launch_direct<1, 1, 4>(a, st);
+}
+
+// Which kernel (us on MI355X, f16 results):
+//   direct  up to 2^20 outputs: its time grows with the work from 2.5 us on (about 280 TOP/s), that of
+//           a single round of tiles is 3.6 + 0.44 per 64 of depth whatever there is to do
+//           (T = 512, N = 2304, K = 768: 9.9, tiles 9.4; T = 256: 6.9, tiles 9.2; T = 1000, N = 1024,
+//           K = 4096: 24.8, tiles 30.6; T = 512: 14.4, tiles 31)
 //   stream  from 256 tiles of 256 x 256 (a tile per CU) at a depth of 1024: below, the steps between
 //           tiles weigh more than the traffic that the larger tile saves (T = 65536, N = 4096,
-//           K = 1024: 340, tiles 446; T = 65536, N = 1024, K = 4096: 257, tiles 311; T = 21853,
-//           N = 2304, K = 768: 64, tiles 58; T = 32768, N = 1152, K = 384: 34, tiles 30)
+//           K = 1024: 336, tiles 446; T = 65536, N = 1024, K = 4096: 257, tiles 311; T = 21853,
+//           N = 768, K = 768: 30, tiles 27; T = 32768, N = 1152, K = 384: 33, tiles 30)
 //   tiles   otherwise
 int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
-  // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens
+  // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens (w: whole tiles too)
   const int64_t most = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
-  const bool near = most > 0 && a.N * a.ldw <= INT32_MAX;
-  if (!near || (int64_t)((a.N + 127) / 128) * ((a.T + 255) / 256) < 32) {
-    const int64_t fb = (a.N + 15) / 16;
-    if (fb * ((a.T + 63) / 64) >= 256) return launch_direct<4, 4>(a, st);
-    if (fb * ((a.T + 31) / 32) >= 256) return launch_direct<2, 4>(a, st);
-    return launch_direct<1, 4>(a, st);
-  }
+  const bool near = most > 0 && (((int64_t)a.N + 255) & ~255ll) * a.ldw <= INT32_MAX;
+  if (!near || (int64_t)a.T * a.N <= 1 << 20) return launch_direct_for(a, st);
   for (int64_t t = 0; t < a.T; t += most) {
     I8LinearArgs c = a;
     c.T = (int)std::min<int64_t>(most, a.T - t);

@@ -26,7 +26,7 @@ from ._lib import (HCR_ACT_GELU, HCR_ACT_NONE, HCR_BF16, HCR_F16, HCR_F32, HCR_N
 _DTYPE = {torch.float16: HCR_F16, torch.bfloat16: HCR_BF16, torch.float32: HCR_F32}
 _ACT = {"none": HCR_ACT_NONE, "gelu": HCR_ACT_GELU}
 _NORM = {"layer": HCR_NORM_LAYER, "rms": HCR_NORM_RMS}
-_I8, _F32 = torch.int8, torch.float32
+_I8, _F32, _Tensor = torch.int8, torch.float32, torch.Tensor
 _grad_on = torch.is_grad_enabled
 _current_device = torch._C._cuda_getDevice            # (torch.cuda.current_device without its init check:
 _current_stream = torch._C._cuda_getCurrentRawStream  # the operands are device tensors; 0.1 us against 1.4)
@@ -36,8 +36,8 @@ _new = object.__new__
 # A single token's call is bound by what the host does, so the checks are one expression per
 # operand; the error message is put together only when it fails.
 def _ok(t, dtypes, dim: int, device: int) -> bool:
-    return (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and t.get_device() == device
-            and device >= 0 and (t.shape[-1] <= 1 or t.stride(-1) == 1)
+    return (isinstance(t, _Tensor) and t.dtype in dtypes and t.dim() == dim and t.get_device() == device >= 0
+            and (t.is_contiguous() or t.shape[-1] <= 1 or t.stride(-1) == 1)
             and not (t.requires_grad and _grad_on()))
 
 
@@ -95,9 +95,10 @@ class Int8Rows:
         device = _device(q, "q", (_I8,), 2)
         if not _ok(scale, (_F32,), 1, device):
             _refuse(scale, "scale", (_F32,), 1, device)
-        if scale.shape[0] != q.shape[0]:
-            raise ValueError(f"{q.shape[0]} rows and {scale.shape[0]} scales")
-        if (q.data_ptr() | _ld(q)) & 15:
+        rows, cols = q.shape
+        if len(scale) != rows:
+            raise ValueError(f"{rows} rows and {len(scale)} scales")
+        if (q.data_ptr() | (q.stride(0) if rows > 1 else 0)) & 15:
             raise ValueError("q: rows must start on 16 bytes (aligned storage, row stride a multiple of 16)")
         self.q, self.scale = q, scale
 
@@ -123,7 +124,7 @@ class Int8Rows:
             raise ValueError(f"dtype {dtype} is not supported here")
         q = self.q
         rows, cols = q.shape
-        out = torch.empty((rows, cols), dtype=dtype, device=q.device)
+        out = q.new_empty((rows, cols), dtype=dtype)
         if rows:
             _call(q.get_device(), lib().hcr_dequant_rows_device, q.data_ptr(), _ld(q), self.scale.data_ptr(), rows,
                   cols, out.data_ptr(), _DTYPE[dtype], cols)
@@ -233,7 +234,7 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
         code = _DTYPE.get(dtype)
         if code is None:
             raise ValueError(f"dtype {dtype} is not supported here")
-        out = torch.empty((rows, features), dtype=dtype, device=xq.device)
+        out = xq.new_empty((rows, features), dtype=dtype)
         ldo = features
     else:
         code, ldo = _rows_operand(out, "out", (rows, features), device)
