@@ -18,11 +18,8 @@
 
 namespace hcr {
 
-// MT + 4 fragments of 16 rows each (1 KiB apart), one wait.  Inline asm: a compiler-visible LDS read
+// 4 + 4 fragments of 16 rows each (1 KiB apart), one wait.  Inline asm: a compiler-visible LDS read
 // after the loop's LDS-DMA would get a vmcnt(0) in front of it, draining the ring.
-__device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av)[8], intx4 (&bq)[4]) {
-  v4_read_frags<intx4>(a, b, av, bq);
-}
 __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av)[4], intx4 (&bq)[4]) {
   asm volatile(
       "ds_read_b128 %0, %8\n\t"
@@ -38,6 +35,46 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
         "=&v"(bq[3])
       : "v"(a), "v"(b)
       : "memory");
+}
+
+// 8 + 4 fragments and, while they are under way, the wave's 4 DMA pieces of a later stage (rows v, depth
+// k, to lds + 0 / 8 / 16 / 24 KiB): a piece holds the wave's issue for about as long as a fragment takes
+// to arrive, and before the reads the pieces would add that to the phase (8192^3: 513 us, so 476).
+#define HCR_I8_DMA(V, RS, OFS)                              \
+  "s_add_u32 m0, %[lds], " OFS "\n\t"                       \
+  "s_nop 0\n\t"                                             \
+  "buffer_load_dwordx4 %[" V "], %[" RS "], %[k] offen lds\n\t"
+__device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av)[8], intx4 (&bq)[4], intx4 wrs, intx4 xrs,
+                                              const int (&v)[4], int k, uint32_t lds) {
+  asm volatile(
+      "ds_read_b128 %8, %[b]\n\t"
+      "ds_read_b128 %9, %[b] offset:1024\n\t"
+      "ds_read_b128 %10, %[b] offset:2048\n\t"
+      "ds_read_b128 %11, %[b] offset:3072\n\t"
+      "ds_read_b128 %0, %[a]\n\t"
+      "ds_read_b128 %1, %[a] offset:1024\n\t"
+      "ds_read_b128 %2, %[a] offset:2048\n\t"
+      "ds_read_b128 %3, %[a] offset:3072\n\t"
+      "ds_read_b128 %4, %[a] offset:4096\n\t"
+      "ds_read_b128 %5, %[a] offset:5120\n\t"
+      "ds_read_b128 %6, %[a] offset:6144\n\t"
+      "ds_read_b128 %7, %[a] offset:7168\n\t"
+      HCR_I8_DMA("v0", "wr", "0")
+      HCR_I8_DMA("v1", "wr", "8192")
+      HCR_I8_DMA("v2", "xr", "16384")
+      HCR_I8_DMA("v3", "xr", "24576")
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(av[0]), "=&v"(av[1]), "=&v"(av[2]), "=&v"(av[3]), "=&v"(av[4]), "=&v"(av[5]), "=&v"(av[6]),
+        "=&v"(av[7]), "=&v"(bq[0]), "=&v"(bq[1]), "=&v"(bq[2]), "=&v"(bq[3])
+      : [a] "v"(a), [b] "v"(b), [wr] "s"(wrs), [xr] "s"(xrs), [v0] "v"(v[0]), [v1] "v"(v[1]), [v2] "v"(v[2]),
+        [v3] "v"(v[3]), [k] "s"(k), [lds] "s"(lds)
+      : "memory", "m0", "scc");
+}
+#undef HCR_I8_DMA
+// a raw buffer descriptor for the above
+__device__ __forceinline__ intx4 i8_rsrc(const void* p, int bytes) {
+  const uint64_t u = (uint64_t)uniform_ptr(p);
+  return intx4{(int)(uint32_t)u, (int)((uint32_t)(u >> 32) & 0xFFFFu), __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
 __device__ __forceinline__ void i8_lds_read4(uint32_t a, uint32_t b, float4 (&u)[2], float4 (&v)[2]) {
   asm volatile(
@@ -273,8 +310,9 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
 //     groups issue it in their R(s).  Before phase 2s every wave has waited for its own pieces of
 //     stage s.
 //   * Every wave issues at least NS stores per tile (i8_store_tile), which the vmcnt waits rely on: a
-//     wait for stage s + 1 may leave the pieces of s + 2 and s + 3 and, in a tile's first three
-//     stages, NS of the previous tile's stores, which are newer than the stage waited for.
+//     wait for stage s + 1 may leave the pieces of s + 2 and s + 3 and, in a tile's first two
+//     stages, NS of the previous tile's stores (issued between the pieces of its s + 2 and s + 3),
+//     which are newer than the stage waited for.
 //   * The tile's scales and biases come with its stage 0, into one of 4 buffers (the stream is up to
 //     4 stages ahead of group 1's epilogue: at 2 stages a tile, 2 tiles).
 // Host-checked: K > 64 (2 stages a tile at least).
@@ -323,10 +361,8 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
   // the stream's head: stage is_s of tile is_i, bound for slot is_slot
   int is_s = 0, is_i = 0, is_slot = 0;
   int voff[4];                                         // (rows here, the depth in the scalar part: see above)
-  auto issue_stage = [&]() __attribute__((always_inline)) {
+  auto stage_rows = [&]() __attribute__((always_inline)) {
     const bool live = is_i < my_tiles;
-    // (past the last tile the pieces are still issued, for the waits' counts, but read nothing)
-    const int far = __builtin_amdgcn_readfirstlane(live ? 0 : I8_FAR);
     if (live && is_s == 0) {
       int f0, t0;
       tile_at(is_i, f0, t0);
@@ -340,12 +376,8 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
       dma4(f_rsrc, s + wave * 256, (f0 + (wave & 3) * 64 + lane) * 4, 0);
       if (wave < 4) dma4(sx_rsrc, s + 2 * FT * 4 + wave * 256, (t0 + wave * 64 + lane) * 4, 0);
     }
-    const int kofs = __builtin_amdgcn_readfirstlane(live ? is_s * KB : 0);
-    char* st = ring + __builtin_amdgcn_readfirstlane(is_slot) * STAGE;
-    dma16(w_rsrc, st + wave * 1024, voff[0] | far, kofs);
-    dma16(w_rsrc, st + (wave + 8) * 1024, voff[1] | far, kofs);
-    dma16(x_rsrc, st + A_BYTES + wave * 1024, voff[2] | far, kofs);
-    dma16(x_rsrc, st + A_BYTES + (wave + 8) * 1024, voff[3] | far, kofs);
+  };
+  auto stage_next = [&]() __attribute__((always_inline)) {
     is_slot = (is_slot + 1) & (NST - 1);
     if (++is_s == nsteps) { is_s = 0; ++is_i; }
   };
@@ -369,7 +401,18 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
                          s0 + (2 * FT + wn * 64) * 4);
   };
 
-  for (int i = 0; i < NST - 1; ++i) issue_stage();
+  for (int i = 0; i < NST - 1; ++i) {
+    stage_rows();
+    const int far = __builtin_amdgcn_readfirstlane(is_i < my_tiles ? 0 : I8_FAR);
+    const int kofs = __builtin_amdgcn_readfirstlane(is_i < my_tiles ? is_s * KB : 0);
+    char* st = ring + __builtin_amdgcn_readfirstlane(is_slot) * STAGE;
+    dma16(w_rsrc, st + wave * 1024, voff[0] | far, kofs);
+    dma16(w_rsrc, st + (wave + 8) * 1024, voff[1] | far, kofs);
+    dma16(x_rsrc, st + A_BYTES + wave * 1024, voff[2] | far, kofs);
+    dma16(x_rsrc, st + A_BYTES + (wave + 8) * 1024, voff[3] | far, kofs);
+    stage_next();
+  }
+  const intx4 wrs = i8_rsrc(a.w, (a.N - 1) * (int)a.ldw + kend), xrs = i8_rsrc(a.x, (a.T - 1) * (int)a.ldx + kend);
   clear();
   v3_wait_vmcnt(8);
   v3_barrier();
@@ -377,8 +420,8 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
   int rslot = 0;
   for (int ti = 0; ti < my_tiles; ++ti) {
     for (int s = 0; s < nsteps; ++s) {
-      issue_stage();
-      __builtin_amdgcn_sched_barrier(0);               // the stores stay behind these pieces (the waits' counts)
+      stage_rows();
+      __builtin_amdgcn_sched_barrier(0);
       if (s == 0 && ti) {
         store_tile(ti - 1);
         clear();
@@ -386,13 +429,20 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
       __builtin_amdgcn_sched_barrier(0);
       const char* st = ring + rslot * STAGE;
       intx4 av[8], bq[4];
-      i8_read_frags(lds_addr(st + offA), lds_addr(st + offB), av, bq);
+      // (past the last tile the pieces are still issued, for the waits' counts, but read nothing)
+      const bool live = is_i < my_tiles;
+      const int far = __builtin_amdgcn_readfirstlane(live ? 0 : I8_FAR);
+      const int vo[4] = {voff[0] | far, voff[1] | far, voff[2] | far, voff[3] | far};
+      i8_read_frags(lds_addr(st + offA), lds_addr(st + offB), av, bq, wrs, xrs, vo,
+                    __builtin_amdgcn_readfirstlane(live ? is_s * KB : 0),
+                    __builtin_amdgcn_readfirstlane(lds_addr(ring) + is_slot * STAGE + wave * 1024));
+      stage_next();
       if ((s + 1) * KB > a.K) {
         const int n = a.K - s * KB - fc * 16;
 #pragma unroll
         for (int m = 0; m < 8; ++m) av[m] = i8_keep(av[m], n);
       }
-      const bool stores = ti && s < 3;                 // the previous tile's are newer than stage s + 1
+      const bool stores = ti && s < 2;                 // the previous tile's are newer than stage s + 1
       if (grp) { if (stores) v3_wait_vmcnt(8 + NS); else v3_wait_vmcnt(8); }
       v3_barrier();
       __builtin_amdgcn_sched_barrier(0);
