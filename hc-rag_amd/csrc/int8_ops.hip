@@ -91,10 +91,11 @@ static int launch_direct_for(const I8LinearArgs& a, hipStream_t st) {
 //           a single round of tiles is 3.6 + 0.44 per 64 of depth whatever there is to do
 //           (T = 512, N = 2304, K = 768: 9.9, tiles 9.4; T = 256: 6.9, tiles 9.2; T = 1000, N = 1024,
 //           K = 4096: 24.8, tiles 30.6; T = 512: 14.4, tiles 31)
-//   stream  from 256 tiles of 256 x 256 (a tile per CU) at a depth of 1024: below, the steps between
-//           tiles weigh more than the traffic that the larger tile saves (T = 65536, N = 4096,
-//           K = 1024: 336, tiles 446; T = 65536, N = 1024, K = 4096: 257, tiles 311; T = 21853,
-//           N = 768, K = 768: 30, tiles 27; T = 32768, N = 1152, K = 384: 33, tiles 30)
+//   stream  where its 256 x 256 tiles fill its rounds (one per CU) to 3/4 at a depth of 1024, to 9/10
+//           from 768 on: a round takes 5.6 + 0.88 per 64 of depth, 512 tiles 2 + 1.15 (T = 65536,
+//           N = 4096, K = 1024: 324, tiles 420; T = 8192, N = 2048, K = 2048: 36, tiles 41; T = 65536,
+//           N = 2304, K = 768: 163, tiles 202; 3.02 rounds, T = 21853: 64, tiles 61; 1.34 rounds,
+//           T = 21853, N = 1024, K = 1024: 36, tiles 33)
 //   tiles   otherwise
 int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
   // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens (w: whole tiles too)
@@ -107,7 +108,8 @@ int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
     c.x = a.x + t * a.ldx;
     c.sx = a.sx + t;
     c.out = static_cast<char*>(a.out) + t * a.ldo * i8_size(a.ot);
-    const bool stream = a.K >= 1024 && (int64_t)((a.N + 255) / 256) * ((c.T + 255) / 256) >= 256;
+    const int64_t big = (int64_t)((a.N + 255) / 256) * ((c.T + 255) / 256), slots = (big + 255) / 256 * 256;
+    const bool stream = a.K >= 1024 ? big * 4 >= slots * 3 : a.K >= 768 && big * 10 >= slots * 9;
     if (a.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
     else if (a.ot == HCR_BF16) launch_linear<HCR_BF16>(c, stream, st);
     else launch_linear<HCR_F16>(c, stream, st);
