@@ -87,10 +87,11 @@ static int launch_direct_for(const I8LinearArgs& a, hipStream_t st) {
 }
 
 // Which kernel (us on MI355X, f16 results):
-//   direct  up to 2^20 outputs: its time grows with the work from 2.5 us on (about 280 TOP/s), that of
+//   direct  up to 2^20 outputs of at most 16 MiB of x: its time grows with the work from 2.5 us on (about 280 TOP/s), that of
 //           a single round of tiles is 3.6 + 0.44 per 64 of depth whatever there is to do
 //           (T = 512, N = 2304, K = 768: 9.9, tiles 9.4; T = 256: 6.9, tiles 9.2; T = 1000, N = 1024,
-//           K = 4096: 24.8, tiles 30.6; T = 512: 14.4, tiles 31)
+//           K = 4096: 24.8, tiles 30.6; T = 512: 14.4, tiles 31); many narrow rows are read from memory
+//           once per 32 features (T = 10000, N = 130, K = 4096: 55, tiles 31)
 //   stream  where its 256 x 256 tiles fill its rounds (one per CU) to 3/4 at a depth of 1024, to 9/10
 //           from 768 on: a round takes 5.6 + 0.88 per 64 of depth, 512 tiles 2 + 1.15 (T = 65536,
 //           N = 4096, K = 1024: 324, tiles 420; T = 8192, N = 2048, K = 2048: 36, tiles 41; T = 65536,
@@ -101,7 +102,7 @@ int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
   // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens (w: whole tiles too)
   const int64_t most = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
   const bool near = most > 0 && (((int64_t)a.N + 255) & ~255ll) * a.ldw <= INT32_MAX;
-  if (!near || (int64_t)a.T * a.N <= 1 << 20) return launch_direct_for(a, st);
+  if (!near || ((int64_t)a.T * a.N <= 1 << 20 && (int64_t)a.T * a.K <= 16 << 20)) return launch_direct_for(a, st);
   for (int64_t t = 0; t < a.T; t += most) {
     I8LinearArgs c = a;
     c.T = (int)std::min<int64_t>(most, a.T - t);
