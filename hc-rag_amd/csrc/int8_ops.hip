@@ -98,23 +98,34 @@ static int launch_direct_for(const I8LinearArgs& a, hipStream_t st) {
 //           N = 2304, K = 768: 163, tiles 202; 3.02 rounds, T = 21853: 64, tiles 61; 1.34 rounds,
 //           T = 21853, N = 1024, K = 1024: 36, tiles 33)
 //   tiles   otherwise
+// A last round of at most 1/8 of its tiles is cut off: the tokens that the full rounds do not cover, if
+// they are few enough for the direct kernel, are left to it (T = 21853, N = 2304, K = 768, 3.02 rounds:
+// 56 us, so 51; T = 16400, N = 1024, K = 4096: 92, 66).
 int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
   // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens (w: whole tiles too)
   const int64_t most = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
   const bool near = most > 0 && (((int64_t)a.N + 255) & ~255ll) * a.ldw <= INT32_MAX;
-  if (!near || ((int64_t)a.T * a.N <= 1 << 20 && (int64_t)a.T * a.K <= 16 << 20)) return launch_direct_for(a, st);
-  for (int64_t t = 0; t < a.T; t += most) {
+  auto few = [&](int64_t T) { return T * a.N <= 1 << 20 && T * a.K <= 16 << 20; };
+  for (int64_t t = 0; t < a.T;) {
     I8LinearArgs c = a;
-    c.T = (int)std::min<int64_t>(most, a.T - t);
+    c.T = (int)(near ? std::min<int64_t>(most, a.T - t) : a.T - t);
     c.x = a.x + t * a.ldx;
     c.sx = a.sx + t;
     c.out = static_cast<char*>(a.out) + t * a.ldo * i8_size(a.ot);
-    const int64_t big = (int64_t)((a.N + 255) / 256) * ((c.T + 255) / 256), slots = (big + 255) / 256 * 256;
-    const bool stream = a.K >= 1024 ? big * 4 >= slots * 3 : a.K >= 768 && big * 10 >= slots * 9;
-    if (a.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
-    else if (a.ot == HCR_BF16) launch_linear<HCR_BF16>(c, stream, st);
-    else launch_linear<HCR_F16>(c, stream, st);
-    HIPC(hipGetLastError());
+    if (!near || few(c.T)) {
+      CHECK(launch_direct_for(c, st));
+    } else {
+      const int64_t nf = (a.N + 255) / 256, nt = (c.T + 255) / 256, over = nf * nt % 256;
+      const int64_t full = nf * nt / 256 * 256 / nf * 256;         // tokens that the full rounds cover
+      if (full > 0 && over > 0 && over <= 32 && few(c.T - full)) c.T = (int)full;
+      const int64_t big = nf * ((c.T + 255) / 256), slots = (big + 255) / 256 * 256;
+      const bool stream = a.K >= 1024 ? big * 4 >= slots * 3 : a.K >= 768 && big * 10 >= slots * 9;
+      if (a.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
+      else if (a.ot == HCR_BF16) launch_linear<HCR_BF16>(c, stream, st);
+      else launch_linear<HCR_F16>(c, stream, st);
+      HIPC(hipGetLastError());
+    }
+    t += c.T;
   }
   return HCR_OK;
 }
