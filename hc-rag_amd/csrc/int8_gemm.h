@@ -40,6 +40,9 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
 // 8 + 4 fragments and, while they are under way, the wave's 4 DMA pieces of a later stage (rows v, depth
 // k, to lds + 0 / 8 / 16 / 24 KiB): a piece holds the wave's issue for about as long as a fragment takes
 // to arrive, and before the reads the pieces would add that to the phase (8192^3: 513 us, so 476).
+// (m0, where a piece goes, is a reserved register: the clobber is kept all the same)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 #define HCR_I8_DMA(V, RS, OFS)                              \
   "s_add_u32 m0, %[lds], " OFS "\n\t"                       \
   "s_nop 0\n\t"                                             \
@@ -71,6 +74,7 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
       : "memory", "m0", "scc");
 }
 #undef HCR_I8_DMA
+#pragma clang diagnostic pop
 // a raw buffer descriptor for the above
 __device__ __forceinline__ intx4 i8_rsrc(const void* p, int bytes) {
   const uint64_t u = (uint64_t)uniform_ptr(p);
@@ -120,9 +124,9 @@ __host__ __device__ constexpr int i8_size(int ot) { return ot == HCR_F32 ? 4 : 2
 // quads are exchanged between neighbouring 16-lane rows, after which a lane holds 8 features of a
 // token and a store covers 16 tokens x 64 bytes (f32: 4 features, the same 64 bytes).  The 2 MT
 // (f32: 4 MT) 16-byte buffer stores are unconditional -- what lies outside is dropped by the
-// descriptor -- so that a wave issues that many for every tile; with ODD (a row is no
-// whole number of 16 bytes) the features of its last, partial 16 bytes follow one by one.  (Rows need
-// only their elements' alignment.)  Without the ODD code the stream kernel holds 30 registers less:
+// descriptor -- so that a wave issues that many for every tile; with ODD (a row is no whole number of
+// 16 bytes) the features of its last, partial 16 bytes follow one by one.  (Rows need only their
+// elements' alignment.)  Without the ODD code the stream kernel holds 30 registers less:
 // T = 21853, N = 2304, K = 768 57 us, with it 64.
 // sw, sb, sx: LDS addresses of the wave's w scales, biases and x scales.
 // Measured against staging the tile through LDS for 256-byte stores, with 128 x 256 tiles of 4 waves
@@ -196,14 +200,17 @@ __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_bu
   }
 }
 
-// A workgroup of WM x WN waves per tile of 16 MT WM features x 64 WN tokens; OCC waves per SIMD.
-template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC>
-__global__ void __launch_bounds__(64 * WM * WN, OCC)
+// A workgroup of 8 waves (2 x 4, 64 features x 64 tokens each) per tile of 128 x 256, two workgroups per
+// CU: while one waits for its stage or stores its tile, the other multiplies.  (us at T = 21853,
+// N = 768, K = 768 / T = 2048, N = 1024, K = 4096: 27.4 / 32.6; 4 waves of 128 x 64 29.4 / 40.0; 128 x 128
+// tiles of 4 waves, three a CU, 25.7 / 32.3 but 446 -> 494 at T = 65536, N = 4096, K = 1024; the
+// alternating groups of the kernel below 26.4 / 31.5, and 5 % behind at K = 384.)
+template <int OT, bool ODD>
+__global__ void __launch_bounds__(512, 4)
 int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
-  constexpr int KB = 64, FT = 16 * MT * WM, TT = 64 * WN, NW = WM * WN;
+  constexpr int KB = 64, MT = 4, WM = 2, WN = 4, NST = 3, FT = 16 * MT * WM, TT = 64 * WN, NW = WM * WN;
   constexpr int NA = FT / 16 / NW, NB = TT / 16 / NW;  // W and X pieces per wave and stage
   constexpr int A_BYTES = FT * KB, STAGE = (FT + TT) * KB, D = NST - 1, NPC = NA + NB;
-  static_assert(FT % (16 * NW) == 0 && TT % (16 * NW) == 0, "whole pieces");
   __shared__ __attribute__((aligned(16))) char ring[NST * STAGE];
   __shared__ __attribute__((aligned(16))) float sc[2 * FT + TT];
 
@@ -295,7 +302,7 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
   const __amdgpu_buffer_rsrc_t o_rsrc = __builtin_amdgcn_make_buffer_rsrc(
       uniform_ptr(a.out), (short)0, __builtin_amdgcn_readfirstlane(((a.T - 1) * (int)a.ldo + a.N) * i8_size(OT)), 0x00020000);
   i8_store_tile<OT, MT, ODD>(a, o_rsrc, acc, lane, f0 + wm * 16 * MT, t0 + wn * 64, lds_addr(sc + wm * 16 * MT),
-                        lds_addr(sc + FT + wm * 16 * MT), lds_addr(sc + 2 * FT + wn * 64));
+                             lds_addr(sc + FT + wm * 16 * MT), lds_addr(sc + 2 * FT + wn * 64));
 }
 
 // -------------------------------------------------------------------------------------
@@ -397,8 +404,8 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
     int f0, t0;
     tile_at(i, f0, t0);
     const uint32_t s0 = lds_addr(sc[i & 3]);
-    i8_store_tile<OT, 8, ODD>(a, o_rsrc, acc, lane, f0 + wm * 128, t0 + wn * 64, s0 + wm * 512, s0 + (FT + wm * 128) * 4,
-                         s0 + (2 * FT + wn * 64) * 4);
+    i8_store_tile<OT, 8, ODD>(a, o_rsrc, acc, lane, f0 + wm * 128, t0 + wn * 64, s0 + wm * 512,
+                              s0 + (FT + wm * 128) * 4, s0 + (2 * FT + wn * 64) * 4);
   };
 
   for (int i = 0; i < NST - 1; ++i) {

@@ -55,7 +55,7 @@ template <int OT, bool ODD>
 static void launch_tiles(const I8LinearArgs& a, hipStream_t st) {
   const int nft = (a.N + 127) / 128;
   const int tiles = nft * ((a.T + 255) / 256);
-  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD, 4, 2, 4, 3, 4>), dim3((unsigned)tiles), dim3(512), 0, st, a, nft);
+  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD>), dim3((unsigned)tiles), dim3(512), 0, st, a, nft);
 }
 template <int OT, bool ODD>
 static void launch_stream(const I8LinearArgs& a, hipStream_t st) {
