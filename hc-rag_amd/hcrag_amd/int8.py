@@ -34,11 +34,39 @@ _new = object.__new__
 
 
 # A single token's call is bound by what the host does, so the checks are one expression per
-# operand; the error message is put together only when it fails.
+# operand, the error message is put together only when it fails, and the C functions are looked up
+# once.
 def _ok(t, dtypes, dim: int, device: int) -> bool:
     return (isinstance(t, _Tensor) and t.dtype in dtypes and t.dim() == dim and t.get_device() == device >= 0
             and (t.is_contiguous() or t.shape[-1] <= 1 or t.stride(-1) == 1)
             and not (t.requires_grad and _grad_on()))
+
+
+class _Entry:
+    """A C entry point, called with torch's current stream of ``device`` as its last argument."""
+
+    __slots__ = ("name", "fn")
+
+    def __init__(self, name: str):
+        self.name, self.fn = name, None
+
+    def __call__(self, device: int, *args) -> None:
+        fn = self.fn
+        if fn is None:
+            fn = self.fn = getattr(lib(), self.name)
+        if device == _current_device():
+            rc = fn(*args, _current_stream(device))
+        else:
+            with torch.cuda.device(device):
+                rc = fn(*args, _current_stream(device))
+        if rc:
+            check(rc)
+
+
+_quant = _Entry("hcr_quant_rows_device")
+_norm_quant = _Entry("hcr_norm_quant_rows_device")
+_dequant = _Entry("hcr_dequant_rows_device")
+_linear = _Entry("hcr_int8_linear_device")
 
 
 def _refuse(t, name: str, dtypes, dim: int, device: Optional[int] = None) -> None:
@@ -72,17 +100,6 @@ def _ld(t) -> int:
     return t.stride(0) if rows > 1 else (cols + 15) // 16 * 16
 
 
-def _call(device: int, fn, *args) -> None:
-    """``fn`` with torch's current stream of ``device`` as its last argument."""
-    if device == _current_device():
-        rc = fn(*args, _current_stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _current_stream(device))
-    if rc:
-        check(rc)
-
-
 class Int8Rows:
     """int8 rows with a scale each: ``q`` int8 [rows, cols], ``scale`` float32 [rows]; an element
     stands for ``q * scale``.  Rows start on 16 bytes (``q[:, :cols]`` of a buffer whose row length
@@ -96,8 +113,8 @@ class Int8Rows:
         if not _ok(scale, (_F32,), 1, device):
             _refuse(scale, "scale", (_F32,), 1, device)
         rows, cols = q.shape
-        if len(scale) != rows:
-            raise ValueError(f"{rows} rows and {len(scale)} scales")
+        if scale.shape[0] != rows:
+            raise ValueError(f"{rows} rows and {scale.shape[0]} scales")
         if (q.data_ptr() | (q.stride(0) if rows > 1 else 0)) & 15:
             raise ValueError("q: rows must start on 16 bytes (aligned storage, row stride a multiple of 16)")
         self.q, self.scale = q, scale
@@ -126,8 +143,8 @@ class Int8Rows:
         rows, cols = q.shape
         out = q.new_empty((rows, cols), dtype=dtype)
         if rows:
-            _call(q.get_device(), lib().hcr_dequant_rows_device, q.data_ptr(), _ld(q), self.scale.data_ptr(), rows,
-                  cols, out.data_ptr(), _DTYPE[dtype], cols)
+            _dequant(q.get_device(), q.data_ptr(), _ld(q), self.scale.data_ptr(), rows, cols, out.data_ptr(),
+                     _DTYPE[dtype], cols)
         return out
 
 
@@ -147,8 +164,8 @@ def quantize_rows(x: torch.Tensor, act: str = "none", out: Optional[Int8Rows] = 
         raise ValueError(f"unknown activation {act!r} (none | gelu)")
     rows, cols = x.shape
     out = _int8_out(out, rows, cols, x)
-    _call(device, lib().hcr_quant_rows_device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols, _ACT[act],
-          out.q.data_ptr(), _ld(out.q), out.scale.data_ptr())
+    _quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols, _ACT[act], out.q.data_ptr(), _ld(out.q),
+           out.scale.data_ptr())
     return out
 
 
@@ -194,9 +211,9 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         norm_t, norm_ld = _rows_operand(norm_out, "norm_out", shape, device)
         norm_p = norm_out.data_ptr()
     out = _int8_out(out, rows, cols, x)
-    _call(device, lib().hcr_norm_quant_rows_device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), resid_p, resid_t, resid_ld,
-          rows, cols, _NORM[norm], weight.data_ptr(), bias_p, eps, sum_p, sum_ld, norm_p, norm_t, norm_ld,
-          out.q.data_ptr(), _ld(out.q), out.scale.data_ptr())
+    _norm_quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), resid_p, resid_t, resid_ld, rows, cols, _NORM[norm],
+                weight.data_ptr(), bias_p, eps, sum_p, sum_ld, norm_p, norm_t, norm_ld, out.q.data_ptr(), _ld(out.q),
+                out.scale.data_ptr())
     return out
 
 
@@ -238,8 +255,8 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
         ldo = features
     else:
         code, ldo = _rows_operand(out, "out", (rows, features), device)
-    _call(device, lib().hcr_int8_linear_device, xq.data_ptr(), _ld(xq), x.scale.data_ptr(), rows, wq.data_ptr(),
-          _ld(wq), w.scale.data_ptr(), features, depth, bias_p, out.data_ptr(), code, ldo)
+    _linear(device, xq.data_ptr(), _ld(xq), x.scale.data_ptr(), rows, wq.data_ptr(), _ld(wq), w.scale.data_ptr(),
+            features, depth, bias_p, out.data_ptr(), code, ldo)
     return out
 
 
