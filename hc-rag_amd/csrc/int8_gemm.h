@@ -37,6 +37,20 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
       : "memory");
 }
 
+__device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av)[2], intx4 (&bq)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %6\n\t"
+      "ds_read_b128 %1, %6 offset:1024\n\t"
+      "ds_read_b128 %2, %7\n\t"
+      "ds_read_b128 %3, %7 offset:1024\n\t"
+      "ds_read_b128 %4, %7 offset:2048\n\t"
+      "ds_read_b128 %5, %7 offset:3072\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(av[0]), "=&v"(av[1]), "=&v"(bq[0]), "=&v"(bq[1]), "=&v"(bq[2]), "=&v"(bq[3])
+      : "v"(a), "v"(b)
+      : "memory");
+}
+
 // 8 + 4 fragments and, while they are under way, the wave's 4 DMA pieces of a later stage (rows v, depth
 // k, to lds + 0 / 8 / 16 / 24 KiB): a piece holds the wave's issue for about as long as a fragment takes
 // to arrive, and before the reads the pieces would add that to the phase (8192^3: 513 us, so 476).
@@ -200,15 +214,12 @@ __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_bu
   }
 }
 
-// A workgroup of 8 waves (2 x 4, 64 features x 64 tokens each) per tile of 128 x 256, two workgroups per
-// CU: while one waits for its stage or stores its tile, the other multiplies.  (us at T = 21853,
-// N = 768, K = 768 / T = 2048, N = 1024, K = 4096: 27.4 / 32.6; 4 waves of 128 x 64 29.4 / 40.0; 128 x 128
-// tiles of 4 waves, three a CU, 25.7 / 32.3 but 446 -> 494 at T = 65536, N = 4096, K = 1024; the
-// alternating groups of the kernel below 26.4 / 31.5, and 5 % behind at K = 384.)
-template <int OT, bool ODD>
-__global__ void __launch_bounds__(512, 4)
+// A workgroup of WM x WN waves per tile of 16 MT WM features x 64 WN tokens; OCC waves per SIMD, so that
+// while one workgroup of a CU waits for its stage or stores its tile another multiplies.
+template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC>
+__global__ void __launch_bounds__(64 * WM * WN, OCC)
 int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
-  constexpr int KB = 64, MT = 4, WM = 2, WN = 4, NST = 3, FT = 16 * MT * WM, TT = 64 * WN, NW = WM * WN;
+  constexpr int KB = 64, FT = 16 * MT * WM, TT = 64 * WN, NW = WM * WN;
   constexpr int NA = FT / 16 / NW, NB = TT / 16 / NW;  // W and X pieces per wave and stage
   constexpr int A_BYTES = FT * KB, STAGE = (FT + TT) * KB, D = NST - 1, NPC = NA + NB;
   __shared__ __attribute__((aligned(16))) char ring[NST * STAGE];

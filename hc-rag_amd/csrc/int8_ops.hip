@@ -50,12 +50,28 @@ static int launch_direct(const I8LinearArgs& a, hipStream_t st) {
   HIPC(hipGetLastError());
   return HCR_OK;
 }
-// 128 features x 256 tokens per workgroup of 8 waves (64 x 64 each), two workgroups per CU
+static int64_t tiles_of(const I8LinearArgs& a, int features, int tokens) {
+  return (int64_t)((a.N + features - 1) / features) * ((a.T + tokens - 1) / tokens);
+}
+template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC>
+static void launch_tile(const I8LinearArgs& a, hipStream_t st) {
+  constexpr int FT = 16 * MT * WM, TT = 64 * WN;
+  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD, MT, WM, WN, NST, OCC>), dim3((unsigned)tiles_of(a, FT, TT)),
+                     dim3(64 * WM * WN), 0, st, a, (a.N + FT - 1) / FT);
+}
+// The widest tile that leaves every CU one, down to 64 x 128 (features x tokens; us on MI355X):
+//   64 x 128   4 waves of 32 x 64: a round takes 2.75 + 0.235 per 64 of depth (T = 2000, N = 1024, K = 4096:
+//              18.5, 128 x 128 22.8, 128 x 256 31.1; T = 4000: 30.3, 24.0, 31.7; T = 1000, N = 768, K = 768:
+//              5.7, 6.7, 9.5)
+//   128 x 128  8 waves of 32 x 64
+//   128 x 256  8 waves of 64 x 64, two workgroups per CU (T = 6000, N = 1024, K = 4096: 33.1, 128 x 128 36.6;
+//              T = 21853, N = 768, K = 768: 27.4, 4 waves of 128 x 64 29.4, alternating wave groups as in
+//              the streaming kernel 26.4, but 5 % behind at K = 384)
 template <int OT, bool ODD>
 static void launch_tiles(const I8LinearArgs& a, hipStream_t st) {
-  const int nft = (a.N + 127) / 128;
-  const int tiles = nft * ((a.T + 255) / 256);
-  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD>), dim3((unsigned)tiles), dim3(512), 0, st, a, nft);
+  if (tiles_of(a, 64, 128) <= 256) launch_tile<OT, ODD, 2, 2, 2, 4, 3>(a, st);
+  else if (tiles_of(a, 128, 128) <= 256) launch_tile<OT, ODD, 2, 4, 2, 4, 4>(a, st);
+  else launch_tile<OT, ODD, 4, 2, 4, 3, 4>(a, st);
 }
 template <int OT, bool ODD>
 static void launch_stream(const I8LinearArgs& a, hipStream_t st) {
@@ -87,37 +103,35 @@ static int launch_direct_for(const I8LinearArgs& a, hipStream_t st) {
 }
 
 // Which kernel (us on MI355X, f16 results):
-//   direct  up to 2^20 outputs of at most 16 MiB of x: its time grows with the work from 2.5 us on (about 280 TOP/s), that of
-//           a single round of tiles is 3.6 + 0.44 per 64 of depth whatever there is to do
-//           (T = 512, N = 2304, K = 768: 9.9, tiles 9.4; T = 256: 6.9, tiles 9.2; T = 1000, N = 1024,
-//           K = 4096: 24.8, tiles 30.6; T = 512: 14.4, tiles 31); many narrow rows are read from memory
-//           once per 32 features (T = 10000, N = 130, K = 4096: 55, tiles 31)
+//   direct  up to 2^19 outputs of at most 16 MiB of x: its time grows with the work from 2.6 us on (about
+//           280 TOP/s), that of a round of small tiles is 2.75 + 0.235 per 64 of depth whatever there is
+//           to do (T = 512, N = 768, K = 768: 5.3, tiles 5.6; T = 768: 6.6, 5.6; T = 512, N = 1024, K = 4096:
+//           14.0, 16.9; T = 768: 24.4, 17.6); many narrow rows are read from memory once per 32 features
+//           (T = 10000, N = 130, K = 4096: 55, tiles 31)
 //   stream  where its 256 x 256 tiles fill its rounds (one per CU) to 3/4 at a depth of 1024, to 9/10
 //           from 768 on: a round takes 5.6 + 0.88 per 64 of depth, 512 tiles 2 + 1.15 (T = 65536,
 //           N = 4096, K = 1024: 324, tiles 420; T = 8192, N = 2048, K = 2048: 36, tiles 41; T = 65536,
-//           N = 2304, K = 768: 163, tiles 202; 3.02 rounds, T = 21853: 64, tiles 61; 1.34 rounds,
-//           T = 21853, N = 1024, K = 1024: 36, tiles 33)
+//           N = 2304, K = 768: 163, tiles 202; 1.34 rounds, T = 21853, N = 1024, K = 1024: 36, tiles 33)
 //   tiles   otherwise
-// A last round of at most 1/8 of its tiles is cut off: the tokens that the full rounds do not cover, if
-// they are few enough for the direct kernel, are left to it (T = 21853, N = 2304, K = 768, 3.02 rounds:
-// 56 us, so 51; T = 16400, N = 1024, K = 4096: 92, 66).
+// A last round of at most 1/4 of its tiles is cut off: the tokens that the full rounds do not cover are
+// a product of their own (T = 21853, N = 2304, K = 768, 3.02 rounds: 56 us, so 51; T = 16400, N = 1024,
+// K = 4096: 92, 66).
 int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
   // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens (w: whole tiles too)
   const int64_t most = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
   const bool near = most > 0 && (((int64_t)a.N + 255) & ~255ll) * a.ldw <= INT32_MAX;
-  auto few = [&](int64_t T) { return T * a.N <= 1 << 20 && T * a.K <= 16 << 20; };
   for (int64_t t = 0; t < a.T;) {
     I8LinearArgs c = a;
     c.T = (int)(near ? std::min<int64_t>(most, a.T - t) : a.T - t);
     c.x = a.x + t * a.ldx;
     c.sx = a.sx + t;
     c.out = static_cast<char*>(a.out) + t * a.ldo * i8_size(a.ot);
-    if (!near || few(c.T)) {
+    if (!near || ((int64_t)c.T * a.N <= 1 << 19 && (int64_t)c.T * a.K <= 16 << 20)) {
       CHECK(launch_direct_for(c, st));
     } else {
       const int64_t nf = (a.N + 255) / 256, nt = (c.T + 255) / 256, over = nf * nt % 256;
       const int64_t full = nf * nt / 256 * 256 / nf * 256;         // tokens that the full rounds cover
-      if (full > 0 && over > 0 && over <= 32 && few(c.T - full)) c.T = (int)full;
+      if (full > 0 && over > 0 && over <= 64 && full < c.T) c.T = (int)full;
       const int64_t big = nf * ((c.T + 255) / 256), slots = (big + 255) / 256 * 256;
       const bool stream = a.K >= 1024 ? big * 4 >= slots * 3 : a.K >= 768 && big * 10 >= slots * 9;
       if (a.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
