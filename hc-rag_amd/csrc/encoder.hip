@@ -53,8 +53,8 @@ struct EncWork {
   DevBuf q8, s8;                          // HCR_I8: the int8 rows under way and their scales
   DevBuf split_ws, split_cnt;             // split GEMM last-round K-split: chunk slabs and a
                                           // ticket counter per tile (zeroed once, reset by use)
-  hipStream_t st = nullptr;               // (split sub-batches only; the first runs unsplit
-  hipEvent_t done = nullptr;              //  batches on the caller's stream)
+  hipStream_t st = nullptr;               // (the first runs on the caller's stream)
+  hipEvent_t done = nullptr;
   bool whole_tiles = false;               // split GEMM in whole-tile rounds only: set when the
                                           // other sub-batch's stream fills the partly filled
                                           // last rounds (reference-precision mode, r06)
@@ -837,8 +837,9 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   const int splits = (want <= 1 || n < kEncSplitMinSeqs) ? 1 : kEncSplits;
   for (EncWork& w : e->work) w.whole_tiles = splits > 1 && e->dtype == HCR_F32;
   if (splits == 1) return run(e->work[0], 0, n, st);
-  // Sub-batches of n / splits sequences, each on a stream of its own (ordered after the caller's
-  // work through ev_in; the caller's stream waits for every sub-batch's `done` event): every
+  // Sub-batches of n / splits sequences, the first on the caller's stream, the others on streams of
+  // their own (ordered after the caller's work through ev_in; the caller's stream waits for their
+  // `done` events): every
   // kernel of a sub-batch is a small grid whose partly filled last round of workgroups the other
   // sub-batch's kernels fill, instead of leaving CUs idle.  Row-wise work and attention within a
   // sequence do not depend on the split, so the embeddings are the same bits.
@@ -846,17 +847,21 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   HIPC(hipEventRecord(e->ev_in, st));
   for (int i = 0; i < splits; ++i) {
     EncWork& w = e->work[i];
-    if (!w.st) {
-      // default priority: work on streams of different priorities has hung MI355X boards
-      HIPC(hipStreamCreateWithFlags(&w.st, hipStreamNonBlocking));
-    }
-    if (!w.done) HIPC(hipEventCreateWithFlags(&w.done, hipEventDisableTiming));
-    HIPC(hipStreamWaitEvent(w.st, e->ev_in, 0));
     const int64_t s0 = n * i / splits, s1 = n * (i + 1) / splits;
+    if (!w.done) HIPC(hipEventCreateWithFlags(&w.done, hipEventDisableTiming));
+    if (i == 0) {
+      HIPC(hipStreamWaitEvent(st, w.done, 0));          // (the last call's stream may be another)
+      CHECK(run(w, s0, s1 - s0, st));
+      HIPC(hipEventRecord(w.done, st));
+      continue;
+    }
+    // default priority: work on streams of different priorities has hung MI355X boards
+    if (!w.st) HIPC(hipStreamCreateWithFlags(&w.st, hipStreamNonBlocking));
+    HIPC(hipStreamWaitEvent(w.st, e->ev_in, 0));
     CHECK(run(w, s0, s1 - s0, w.st));
     HIPC(hipEventRecord(w.done, w.st));
+    HIPC(hipStreamWaitEvent(st, w.done, 0));
   }
-  for (int i = 0; i < splits; ++i) HIPC(hipStreamWaitEvent(st, e->work[i].done, 0));
   return HCR_OK;
 }
 
