@@ -16,7 +16,7 @@ struct I8RowArgs {
   const float* g; const float* b;  // (b NULL: 0)
   int8_t* q; int64_t ldq;
   float* scale;
-  int64_t rows;
+  int64_t rows, row0;              // rows [row0, row0 + rows) (the host cuts very long calls)
   int cols;
   float eps;
   int xt, rt, yt;                  // hcr_dtype of x, r (and sum), y

@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 rows_to_int8_kernel(I8RowArgs a) {
   __shared__ uint32_t red[WAVES > 1 ? WAVES : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
-  if (WAVES == 1 && row >= a.rows) return;
+  const unsigned at = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  if (WAVES == 1 && at >= a.rows) return;
+  const int64_t row = a.row0 + at;
   const int tid = WAVES == 1 ? lane : threadIdx.x;
   constexpr int NTH = 64 * WAVES;
   constexpr bool NORM = MODE == I8_LAYER || MODE == I8_RMS;
@@ -345,10 +346,9 @@ __global__ void __launch_bounds__(256)
 int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, unsigned rows,
                     int cols, void* __restrict__ out, int ot, int64_t ldo) {
   const unsigned per = (unsigned)(cols + 7) >> 3;
-  const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const unsigned row = id >> 32 ? (unsigned)(id / per) : (unsigned)id / per;   // (the 64-bit one is long)
+  const unsigned id = blockIdx.x * 256 + threadIdx.x, row = id / per;            // (the host: below 2^32)
   if (row >= rows) return;
-  const int i = min((int)(unsigned)(id - (uint64_t)row * per) * 8, max(cols - 8, 0));
+  const int i = min((int)(id - row * per) * 8, max(cols - 8, 0));
   const int8_t* qr = q + row * ldq + i;
   char* orow = reinterpret_cast<char*>(out) + row * ldo * (ot == HCR_F32 ? 4 : 2);
   const float s = scale[row];

@@ -9,6 +9,7 @@ struct I8RowArgs;
 struct I8LinearArgs;
 constexpr int kI8MaxRowCols = 32768;       // 16 waves x 4 chunks x 512 elements
 constexpr int kI8MaxRows = 1 << 30;        // rows and features (32-bit row indices)
+constexpr int64_t kI8MaxElements = (int64_t)1 << 40;   // of a product's or a dequantisation's result
 constexpr int kI8MaxDepth = 131071;        // 2^14 K < 2^31: the int32 sums stay exact
 int int8_rows_launch(int mode, const I8RowArgs& a, hipStream_t st);
 int int8_linear_launch(const I8LinearArgs& a, hipStream_t st);

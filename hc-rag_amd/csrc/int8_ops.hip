@@ -12,11 +12,19 @@ using namespace hcr;
 
 namespace hcr {
 
+constexpr int64_t kLaunchThreads = (int64_t)1 << 31;   // per launch; a grid of 2^32 threads is refused
+
 template <int MODE, int WAVES, int NCH>
 static void launch_rows(const I8RowArgs& a, hipStream_t st) {
-  const unsigned grid = WAVES == 1 ? (unsigned)((a.rows + 3) / 4) : (unsigned)a.rows;
-  hipLaunchKernelGGL((rows_to_int8_kernel<MODE, WAVES, NCH>), dim3(grid), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0,
-                     st, a);
+  constexpr int64_t most = kLaunchThreads / (64 * WAVES);        // rows per launch
+  for (int64_t r = 0; r < a.rows; r += most) {
+    I8RowArgs c = a;
+    c.row0 = r;
+    c.rows = std::min(most, a.rows - r);
+    const unsigned grid = WAVES == 1 ? (unsigned)((c.rows + 3) / 4) : (unsigned)c.rows;
+    hipLaunchKernelGGL((rows_to_int8_kernel<MODE, WAVES, NCH>), dim3(grid), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0,
+                       st, c);
+  }
 }
 // The narrowest layout that holds a row.  Up to 2048 columns a wave per row (a workgroup per row
 // pays its barriers three times: 60000 x 384 LayerNorm 45 us, 89 with 4 waves a row; 65536 x 2048
@@ -45,7 +53,6 @@ int int8_rows_launch(int mode, const I8RowArgs& a, hipStream_t st) {
 template <int FB, int TB, int KW>
 static int launch_direct(const I8LinearArgs& a, hipStream_t st) {
   const int64_t blocks = (int64_t)((a.N + 16 * FB - 1) / (16 * FB)) * ((a.T + 16 * TB - 1) / (16 * TB));
-  if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many outputs for one call");
   hipLaunchKernelGGL((int8_linear_direct<FB, TB, KW>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
   HIPC(hipGetLastError());
   return HCR_OK;
@@ -117,29 +124,38 @@ static int launch_direct_for(const I8LinearArgs& a, hipStream_t st) {
 // a product of their own (T = 21853, N = 2304, K = 768, 3.02 rounds: 56 us, so 51; T = 16400, N = 1024,
 // K = 4096: 92, 66).
 int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
-  // rows of x and out that 31-bit byte offsets reach, in whole tiles of tokens (w: whole tiles too)
-  const int64_t most = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
-  const bool near = most > 0 && (((int64_t)a.N + 255) & ~255ll) * a.ldw <= INT32_MAX;
-  for (int64_t t = 0; t < a.T;) {
+  // rows of w, x and out that 31-bit byte offsets reach, in whole tiles
+  const int64_t fmost = INT32_MAX / a.ldw / 256 * 256;
+  const int64_t tmost = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
+  const bool near = fmost > 0 && tmost > 0;
+  const int64_t fstep = std::min<int64_t>(near ? fmost : a.N, 1 << 22);
+  // (far: the direct kernel's offsets have 64 bits; at most max(2^30, 512 * 2^22) threads a launch)
+  const int64_t tstep = near ? tmost : std::max<int64_t>((1 << 30) / std::min<int64_t>(a.N, fstep) / 64 * 64, 512);
+  for (int64_t f = 0; f < a.N; f += fstep) {
     I8LinearArgs c = a;
-    c.T = (int)(near ? std::min<int64_t>(most, a.T - t) : a.T - t);
-    c.x = a.x + t * a.ldx;
-    c.sx = a.sx + t;
-    c.out = static_cast<char*>(a.out) + t * a.ldo * i8_size(a.ot);
-    if (!near || ((int64_t)c.T * a.N <= 1 << 19 && (int64_t)c.T * a.K <= 16 << 20)) {
-      CHECK(launch_direct_for(c, st));
-    } else {
-      const int64_t nf = (a.N + 255) / 256, nt = (c.T + 255) / 256, over = nf * nt % 256;
+    c.N = (int)std::min(fstep, a.N - f);
+    c.w = a.w + f * a.ldw;
+    c.sw = a.sw + f;
+    if (a.bias) c.bias = a.bias + f;
+    for (int64_t t = 0; t < a.T; t += c.T) {
+      c.T = (int)std::min(tstep, a.T - t);
+      c.x = a.x + t * a.ldx;
+      c.sx = a.sx + t;
+      c.out = static_cast<char*>(a.out) + (t * a.ldo + f) * i8_size(a.ot);
+      if (!near || ((int64_t)c.T * c.N <= 1 << 19 && (int64_t)c.T * c.K <= 16 << 20)) {
+        CHECK(launch_direct_for(c, st));
+        continue;
+      }
+      const int64_t nf = (c.N + 255) / 256, nt = (c.T + 255) / 256, over = nf * nt % 256;
       const int64_t full = nf * nt / 256 * 256 / nf * 256;         // tokens that the full rounds cover
       if (full > 0 && over > 0 && over <= 64 && full < c.T) c.T = (int)full;
       const int64_t big = nf * ((c.T + 255) / 256), slots = (big + 255) / 256 * 256;
-      const bool stream = a.K >= 1024 ? big * 4 >= slots * 3 : a.K >= 768 && big * 10 >= slots * 9;
-      if (a.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
-      else if (a.ot == HCR_BF16) launch_linear<HCR_BF16>(c, stream, st);
+      const bool stream = c.K >= 1024 ? big * 4 >= slots * 3 : c.K >= 768 && big * 10 >= slots * 9;
+      if (c.ot == HCR_F32) launch_linear<HCR_F32>(c, stream, st);
+      else if (c.ot == HCR_BF16) launch_linear<HCR_BF16>(c, stream, st);
       else launch_linear<HCR_F16>(c, stream, st);
       HIPC(hipGetLastError());
     }
-    t += c.T;
   }
   return HCR_OK;
 }
@@ -151,24 +167,34 @@ static bool is_float(int dt) { return dt == HCR_F16 || dt == HCR_BF16 || dt == H
 static bool on(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // a [rows][cols] operand of a floating type: its type, stride and alignment
-static int check_floats(const char* what, const void* p, int dt, int64_t ld, int cols) {
+static int check_floats(const char* what, const void* p, int dt, int64_t ld, int64_t cols) {
   if (!is_float(dt)) return hcr_set_errorf(HCR_EINVAL, "%s: dtype must be HCR_F16, HCR_BF16 or HCR_F32, got %d", what, dt);
-  if (ld < cols) return hcr_set_errorf(HCR_EINVAL, "%s: row stride %lld is below %d columns", what, (long long)ld, cols);
+  if (ld < cols) return hcr_set_errorf(HCR_EINVAL, "%s: row stride %lld is below %lld columns", what, (long long)ld, (long long)cols);
   if (!on(p, float_size(dt))) return hcr_set_errorf(HCR_EINVAL, "%s: not aligned to its elements", what);
   return HCR_OK;
 }
-static int check_int8(const char* what, const void* p, int64_t ld, int cols) {
-  if (ld < cols) return hcr_set_errorf(HCR_EINVAL, "%s: row stride %lld is below %d columns", what, (long long)ld, cols);
+static int check_int8(const char* what, const void* p, int64_t ld, int64_t cols) {
+  if (ld < cols) return hcr_set_errorf(HCR_EINVAL, "%s: row stride %lld is below %lld columns", what, (long long)ld, (long long)cols);
   if (!on(p, 16) || (ld & 15))
     return hcr_set_errorf(HCR_EINVAL, "%s: int8 rows must start on 16 bytes (aligned pointer, row stride a multiple of 16)", what);
   return HCR_OK;
 }
-static int check_rows(int64_t rows, int cols, int64_t max_cols) {
+static int check_rows(int64_t rows, int64_t cols, int64_t max_cols) {
   if (rows < 0 || rows > kI8MaxRows) return hcr_set_errorf(HCR_EINVAL, "rows must be in [0, 2^30], got %lld", (long long)rows);
-  if (cols < 1 || cols > max_cols) return hcr_set_errorf(HCR_EINVAL, "cols must be in [1, %lld], got %d", (long long)max_cols, cols);
+  if (cols < 1 || cols > max_cols) return hcr_set_errorf(HCR_EINVAL, "cols must be in [1, %lld], got %lld", (long long)max_cols, (long long)cols);
   return HCR_OK;
 }
-extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int cols, int act,
+// rows in one buffer as another operand's: the same element for element, or refused
+static int check_same(const char* what, const void* p, int dt, int64_t ld, const char* other, const void* o, int odt, int64_t old) {
+  if (p && p == o && (dt != odt || ld != old))
+    return hcr_set_errorf(HCR_EINVAL, "%s in the buffer of %s: needs its dtype and row stride", what, other);
+  return HCR_OK;
+}
+static int check_apart(const char* what, const void* p, const char* other, const void* o) {
+  return p && p == o ? hcr_set_errorf(HCR_EINVAL, "%s and %s must not overlap", what, other) : HCR_OK;
+}
+
+extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, int act,
                                      int8_t* d_q, int64_t ldq, float* d_scale, void* stream) {
   CHECK(check_rows(rows, cols, kI8MaxRowCols));
   if (act != HCR_ACT_NONE && act != HCR_ACT_GELU) return hcr_set_errorf(HCR_EINVAL, "unknown activation %d", act);
@@ -177,14 +203,15 @@ extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, 
   CHECK(check_floats("x", d_x, x_dtype, ldx, cols));
   CHECK(check_int8("q", d_q, ldq, cols));
   if (!on(d_scale, 4)) return hcr_set_error(HCR_EINVAL, "scale: not aligned to its elements");
+  CHECK(check_apart("q", d_q, "x", d_x));
   I8RowArgs a{};
   a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
-  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = cols;
+  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = (int)cols;
   return int8_rows_launch(act == HCR_ACT_GELU ? I8_GELU : I8_QUANT, a, (hipStream_t)stream);
 }
 
 extern "C" int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, const void* d_residual,
-                                          int r_dtype, int64_t ldr, int64_t rows, int cols, int norm,
+                                          int r_dtype, int64_t ldr, int64_t rows, int64_t cols, int norm,
                                           const float* d_weight, const float* d_bias, float eps, void* d_sum,
                                           int64_t ldsum, void* d_norm, int norm_dtype, int64_t ldnorm, int8_t* d_q,
                                           int64_t ldq, float* d_scale, void* stream) {
@@ -201,17 +228,26 @@ extern "C" int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t 
   CHECK(check_int8("q", d_q, ldq, cols));
   if (!on(d_scale, 4) || !on(d_weight, 4) || !on(d_bias, 4))
     return hcr_set_error(HCR_EINVAL, "scale, weight or bias: not aligned to its elements");
+  CHECK(check_same("the sum", d_sum, r_dtype, ldsum, "the residual", d_residual, r_dtype, ldr));
+  CHECK(check_same("the norm output", d_norm, norm_dtype, ldnorm, "x", d_x, x_dtype, ldx));
+  CHECK(check_same("the norm output", d_norm, norm_dtype, ldnorm, "the residual", d_residual, r_dtype, ldr));
+  CHECK(check_apart("the sum", d_sum, "x", d_x));
+  CHECK(check_apart("the sum", d_sum, "the norm output", d_norm));
+  CHECK(check_apart("q", d_q, "x", d_x));
+  CHECK(check_apart("q", d_q, "the residual", d_residual));
+  CHECK(check_apart("q", d_q, "the sum", d_sum));
+  CHECK(check_apart("q", d_q, "the norm output", d_norm));
   I8RowArgs a{};
   a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
   a.r = d_residual; a.ldr = ldr; a.rt = d_residual ? r_dtype : HCR_F32;
   a.sum = d_sum; a.ldsum = ldsum;
   a.y = d_norm; a.ldy = ldnorm; a.yt = norm_dtype;
   a.g = d_weight; a.b = d_bias; a.eps = eps;
-  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = cols;
+  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = (int)cols;
   return int8_rows_launch(norm == HCR_NORM_LAYER ? I8_LAYER : I8_RMS, a, (hipStream_t)stream);
 }
 
-extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows, int cols,
+extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows, int64_t cols,
                                        void* d_out, int out_dtype, int64_t ldo, void* stream) {
   CHECK(check_rows(rows, cols, kI8MaxDepth));
   if (rows == 0) return HCR_OK;
@@ -219,20 +255,26 @@ extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const flo
   CHECK(check_int8("q", d_q, ldq, cols));
   CHECK(check_floats("out", d_out, out_dtype, ldo, cols));
   if (!on(d_scale, 4)) return hcr_set_error(HCR_EINVAL, "scale: not aligned to its elements");
-  const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
-  if (blocks > INT32_MAX) return hcr_set_error(HCR_EINVAL, "too many elements for one call");
-  hipLaunchKernelGGL(int8_to_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, ldq,
-                     d_scale, (unsigned)rows, cols, d_out, out_dtype, ldo);
-  HIPC(hipGetLastError());
+  CHECK(check_apart("out", d_out, "q", d_q));
+  if (rows * cols > kI8MaxElements) return hcr_set_error(HCR_EINVAL, "more than 2^40 elements");
+  const int64_t per = (cols + 7) / 8, most = kLaunchThreads / per;   // threads per row, rows per launch
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = std::min(most, rows - r);
+    hipLaunchKernelGGL(int8_to_rows_kernel, dim3((unsigned)((n * per + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                       d_q + r * ldq, ldq, d_scale + r, (unsigned)n, (int)cols,
+                       static_cast<char*>(d_out) + r * ldo * (int64_t)float_size(out_dtype), out_dtype, ldo);
+    HIPC(hipGetLastError());
+  }
   return HCR_OK;
 }
 
 extern "C" int hcr_int8_linear_device(const int8_t* d_x, int64_t ldx, const float* d_x_scale, int64_t rows,
-                                      const int8_t* d_w, int64_t ldw, const float* d_w_scale, int features, int depth,
-                                      const float* d_bias, void* d_out, int out_dtype, int64_t ldo, void* stream) {
+                                      const int8_t* d_w, int64_t ldw, const float* d_w_scale, int64_t features,
+                                      int64_t depth, const float* d_bias, void* d_out, int out_dtype, int64_t ldo,
+                                      void* stream) {
   CHECK(check_rows(rows, depth, kI8MaxDepth));
   if (features < 0 || features > kI8MaxRows)
-    return hcr_set_errorf(HCR_EINVAL, "features must be in [0, 2^30], got %d", features);
+    return hcr_set_errorf(HCR_EINVAL, "features must be in [0, 2^30], got %lld", (long long)features);
   if (rows == 0 || features == 0) return HCR_OK;
   if (!d_x || !d_x_scale || !d_w || !d_w_scale || !d_out) return hcr_set_error(HCR_EINVAL, "NULL buffer");
   CHECK(check_int8("x", d_x, ldx, depth));
@@ -240,11 +282,14 @@ extern "C" int hcr_int8_linear_device(const int8_t* d_x, int64_t ldx, const floa
   CHECK(check_floats("out", d_out, out_dtype, ldo, features));
   if (!on(d_x_scale, 4) || !on(d_w_scale, 4) || !on(d_bias, 4))
     return hcr_set_error(HCR_EINVAL, "scales or bias: not aligned to their elements");
+  CHECK(check_apart("out", d_out, "x", d_x));
+  CHECK(check_apart("out", d_out, "w", d_w));
+  if (rows * features > kI8MaxElements) return hcr_set_error(HCR_EINVAL, "more than 2^40 outputs");
   I8LinearArgs a{};
   a.x = d_x; a.ldx = ldx; a.sx = d_x_scale;
   a.w = d_w; a.ldw = ldw; a.sw = d_w_scale;
   a.bias = d_bias; a.out = d_out; a.ldo = ldo; a.ot = out_dtype;
-  a.T = (int)rows; a.N = features; a.K = depth;
+  a.T = (int)rows; a.N = (int)features; a.K = (int)depth;
   a.vec = ldo % 4 == 0 && on(d_out, 4 * float_size(out_dtype));
   return int8_linear_launch(a, (hipStream_t)stream);
 }

@@ -101,17 +101,17 @@ _SIGS = {
     "hcr_encode": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "hcr_encode_device": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
                                   c_void_p]),
-    "hcr_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
+    "hcr_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p,
                                       c_int64, c_void_p, c_void_p]),
     "hcr_norm_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
-                                           c_int64, c_int, c_int, c_void_p, c_void_p, c_float,
+                                           c_int64, c_int64, c_int, c_void_p, c_void_p, c_float,
                                            c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p,
                                            c_int64, c_void_p, c_void_p]),
-    "hcr_dequant_rows_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+    "hcr_dequant_rows_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                         c_int, c_int64, c_void_p]),
     "hcr_int8_linear_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
-                                       c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int64,
-                                       c_void_p]),
+                                       c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int,
+                                       c_int64, c_void_p]),
     "hcr_relevance_combine": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int, c_int64,
                                       c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                       c_void_p, c_int, c_int, c_void_p, c_int, c_void_p,

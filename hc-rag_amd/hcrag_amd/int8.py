@@ -106,7 +106,9 @@ class Int8Rows:
     is a multiple of 16); what lies between a row's end and the next row is never read as a value.
     """
 
-    __slots__ = ("q", "scale")
+    __slots__ = ("_q", "_scale")
+    q = property(lambda self: self._q)
+    scale = property(lambda self: self._scale)
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         device = _device(q, "q", (_I8,), 2)
@@ -117,33 +119,33 @@ class Int8Rows:
             raise ValueError(f"{rows} rows and {scale.shape[0]} scales")
         if (q.data_ptr() | (q.stride(0) if rows > 1 else 0)) & 15:
             raise ValueError("q: rows must start on 16 bytes (aligned storage, row stride a multiple of 16)")
-        self.q, self.scale = q, scale
+        self._q, self._scale = q, scale
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Int8Rows":
         """Uninitialised rows, laid out as the operators want them."""
         self = _new(cls)
-        self.q = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=_I8, device=device)
-        self.scale = torch.empty(rows, dtype=_F32, device=device)
+        self._q = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=_I8, device=device)
+        self._scale = torch.empty(rows, dtype=_F32, device=device)
         return self
 
     @property
     def shape(self):
-        return self.q.shape
+        return self._q.shape
 
     @property
     def device(self):
-        return self.q.device
+        return self._q.device
 
     def dequantize(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
         """[rows, cols] of the values that the rows stand for, rounded to ``dtype``."""
         if dtype not in _DTYPE:
             raise ValueError(f"dtype {dtype} is not supported here")
-        q = self.q
+        q = self._q
         rows, cols = q.shape
         out = q.new_empty((rows, cols), dtype=dtype)
         if rows:
-            _dequant(q.get_device(), q.data_ptr(), _ld(q), self.scale.data_ptr(), rows, cols, out.data_ptr(),
+            _dequant(q.get_device(), q.data_ptr(), _ld(q), self._scale.data_ptr(), rows, cols, out.data_ptr(),
                      _DTYPE[dtype], cols)
         return out
 
@@ -151,8 +153,8 @@ class Int8Rows:
 def _int8_out(out: Optional[Int8Rows], rows: int, cols: int, like: torch.Tensor) -> Int8Rows:
     if out is None:
         return Int8Rows.empty(rows, cols, like.device)
-    if tuple(out.q.shape) != (rows, cols) or out.q.device != like.device:
-        raise ValueError(f"out: {tuple(out.q.shape)} on {out.q.device}, expected {(rows, cols)} on {like.device}")
+    if tuple(out._q.shape) != (rows, cols) or out._q.device != like.device:
+        raise ValueError(f"out: {tuple(out._q.shape)} on {out._q.device}, expected {(rows, cols)} on {like.device}")
     return out
 
 
@@ -164,8 +166,8 @@ def quantize_rows(x: torch.Tensor, act: str = "none", out: Optional[Int8Rows] = 
         raise ValueError(f"unknown activation {act!r} (none | gelu)")
     rows, cols = x.shape
     out = _int8_out(out, rows, cols, x)
-    _quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols, _ACT[act], out.q.data_ptr(), _ld(out.q),
-           out.scale.data_ptr())
+    _quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols, _ACT[act], out._q.data_ptr(), _ld(out._q),
+           out._scale.data_ptr())
     return out
 
 
@@ -212,8 +214,8 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         norm_p = norm_out.data_ptr()
     out = _int8_out(out, rows, cols, x)
     _norm_quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), resid_p, resid_t, resid_ld, rows, cols, _NORM[norm],
-                weight.data_ptr(), bias_p, eps, sum_p, sum_ld, norm_p, norm_t, norm_ld, out.q.data_ptr(), _ld(out.q),
-                out.scale.data_ptr())
+                weight.data_ptr(), bias_p, eps, sum_p, sum_ld, norm_p, norm_t, norm_ld, out._q.data_ptr(), _ld(out._q),
+                out._scale.data_ptr())
     return out
 
 
@@ -232,7 +234,7 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
     [rows, features] in ``dtype`` (or into ``out``).  The integer sums are exact."""
     if not isinstance(x, Int8Rows) or not isinstance(w, Int8Rows):
         raise ValueError("x and w: expected Int8Rows (quantize_rows makes them)")
-    xq, wq = x.q, w.q
+    xq, wq = x._q, w._q
     rows, depth = xq.shape
     features, depth_w = wq.shape
     device = xq.get_device()
@@ -255,7 +257,7 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
         ldo = features
     else:
         code, ldo = _rows_operand(out, "out", (rows, features), device)
-    _linear(device, xq.data_ptr(), _ld(xq), x.scale.data_ptr(), rows, wq.data_ptr(), _ld(wq), w.scale.data_ptr(),
+    _linear(device, xq.data_ptr(), _ld(xq), x._scale.data_ptr(), rows, wq.data_ptr(), _ld(wq), w._scale.data_ptr(),
             features, depth, bias_p, out.data_ptr(), code, ldo)
     return out
 

@@ -321,8 +321,9 @@ typedef struct hcr_encoder hcr_encoder;
  *   HCR_I8   fastest: the projections as 8-bit integer products (weights with a scale per output
  *            channel, activations with a scale per token, quantised as the int8 operators below
  *            do), f16 attention and product outputs, fp32 LayerNorm, GELU and residual stream.
- *            Quantisation is part of the result: cosine to fp32 BertModel about 0.999, not the
- *            16-bit modes' 0.9999.  Needs intermediate <= 32768. */
+ *            Quantisation is part of the result: cosine to fp32 BertModel >= 0.9999 on seeded
+ *            weights (16-bit modes: 0.999999); trained activations spread wider.  Needs
+ *            intermediate <= 32768. */
 int hcr_encoder_create(int device, const hcr_bert_config* cfg, int compute_dtype,
                        hcr_encoder** out);
 int hcr_encoder_compute_dtype(const hcr_encoder* enc);
@@ -359,7 +360,9 @@ int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_m
  * Asynchronous on `stream` (a hipStream_t of the current device; NULL = the legacy default
  * stream).  Nothing is allocated, waited for or kept between calls: calls may run at once from
  * several threads and be captured into graphs.  0 rows (and 0 features): nothing is done.
- * At most 2^30 rows and features; quantised rows of 1 .. 32768 columns.
+ * At most 2^30 rows and features, and 2^40 elements of a result; quantised rows of 1 .. 32768
+ * columns.  Buffers of a call must not overlap unless said otherwise; outputs that start where
+ * another operand does are refused.
  *
  * Quantisation of a row v: a = max |v|, scale = a / 127, q = round_half_even(v * (127 / a)), in
  * fp32.  a < 2^-100: the row counts as zeros (q 0, scale 0).  A row that holds a NaN or an
@@ -369,7 +372,7 @@ int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_m
 
 /* v = activation(x): int8 rows of x [rows][cols] (x_dtype HCR_F16 / HCR_BF16 / HCR_F32).  Weights
  * [features][depth] are laid out by the same call: a channel is a row. */
-int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int cols,
+int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols,
                           int activation, int8_t* d_q, int64_t ldq, float* d_scale, void* stream);
 
 /* h = x + residual (residual NULL: h = x); v = norm(h) * weight + bias (bias NULL: 0), with
@@ -379,21 +382,21 @@ int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t row
  * d_norm x or the residual itself (same type and stride); other buffers must not overlap.  weight
  * and bias: fp32, cols elements. */
 int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, const void* d_residual,
-                               int r_dtype, int64_t ldr, int64_t rows, int cols, int norm,
+                               int r_dtype, int64_t ldr, int64_t rows, int64_t cols, int norm,
                                const float* d_weight, const float* d_bias, float eps, void* d_sum,
                                int64_t ldsum, void* d_norm, int norm_dtype, int64_t ldnorm,
                                int8_t* d_q, int64_t ldq, float* d_scale, void* stream);
 
 /* out [rows][cols] = q * scale, rounded to out_dtype (1 <= cols <= 131071). */
 int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows,
-                            int cols, void* d_out, int out_dtype, int64_t ldo, void* stream);
+                            int64_t cols, void* d_out, int out_dtype, int64_t ldo, void* stream);
 
-/* out[t][f] = (sum_k x[t][k] w[f][k]) * x_scale[t] * w_scale[f] + bias[f] (bias NULL: 0), x [rows]
+/* out[t][f] = ((sum_k x[t][k] w[f][k]) * x_scale[t]) * w_scale[f] + bias[f] (bias NULL: 0), x [rows]
  * [depth] and w [features][depth] int8 rows.  The sum is exact (int32; 1 <= depth <= 131071), the
- * rest fp32, rounded once to out_dtype. */
+ * rest fp32 in this order, rounded once to out_dtype. */
 int hcr_int8_linear_device(const int8_t* d_x, int64_t ldx, const float* d_x_scale, int64_t rows,
-                           const int8_t* d_w, int64_t ldw, const float* d_w_scale, int features,
-                           int depth, const float* d_bias, void* d_out, int out_dtype, int64_t ldo,
+                           const int8_t* d_w, int64_t ldw, const float* d_w_scale, int64_t features,
+                           int64_t depth, const float* d_bias, void* d_out, int out_dtype, int64_t ldo,
                            void* stream);
 
 /* ---------------------------------------------------------------------------------------

@@ -52,6 +52,32 @@ def test_bad_arguments_are_refused(call, wrong):
     assert _lib.lib().hcr_last_error()
 
 
+# buffers of their own: what is in one place twice is what the case says
+X, R, S, Y, Q, O = (P * (2 + i) for i in range(6))
+OWN = {quant: dict(x=X, q=Q), norm: dict(x=X, r=R, s=S, y=Y, q=Q), dequant: dict(q=Q, out=O),
+       linear: dict(x=X, w=Q, out=O)}
+ALIASED = [
+    (quant, dict(q=X)), (dequant, dict(out=Q)), (linear, dict(out=X)), (linear, dict(out=Q)),
+    (norm, dict(s=R, lds=128)), (norm, dict(y=X, yt=BF16)), (norm, dict(y=X, ldy=128)), (norm, dict(y=R, yt=F16)),
+    (norm, dict(y=R, yt=F32, ldy=128)), (norm, dict(s=X)), (norm, dict(s=Y)), (norm, dict(s=R, y=R, yt=F32)),
+    (norm, dict(q=X)), (norm, dict(q=R)), (norm, dict(q=S)), (norm, dict(q=Y)),
+]
+
+
+@pytest.mark.parametrize("call,wrong", ALIASED, ids=lambda v: getattr(v, "__name__", None) or ",".join(v))
+def test_outputs_in_the_place_of_operands_are_refused(call, wrong):
+    assert call(**{**OWN[call], **wrong}) == _lib.HCR_EINVAL
+    assert b"overlap" in _lib.lib().hcr_last_error() or b"buffer of" in _lib.lib().hcr_last_error()
+
+
+@pytest.mark.parametrize("call,name", [(quant, "cols"), (norm, "cols"), (dequant, "cols"), (linear, "depth"), (linear, "features")])
+def test_sizes_past_32_bits_are_refused_not_cut(call, name):
+    far = 1 << 33
+    strides = {quant: ("ldx", "ldq"), norm: ("ldx", "ldr", "lds", "ldy", "ldq"), dequant: ("ldq", "ldo"),
+               linear: ("ldx", "ldw", "ldo")}[call]
+    assert call(**{**OWN[call], name: (1 << 32) + 8, **{k: far for k in strides}}) == _lib.HCR_EINVAL
+
+
 def test_nothing_to_do_is_ok():
     assert quant(rows=0, x=None, q=None, scale=None) == 0
     assert norm(rows=0, x=None, w=None, q=None, scale=None) == 0

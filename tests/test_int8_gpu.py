@@ -148,6 +148,32 @@ def test_linear_offsets_past_32_bits():
 
 
 @gpu
+def test_linear_more_features_than_one_launch():
+    """Features are cut like tokens: 2^22 of them a launch."""
+    m, g = _ops(), _gen(9)
+    T, N, K = 3, 2 ** 22 + 301, 16
+    x, w = _int8(g, T, K), _int8(g, N, K)
+    sx, sw, b = _scales(g, T), _scales(g, N), torch.randn(N, generator=g, device="cuda")
+    y = m.int8_linear(m.Int8Rows(x, sx), m.Int8Rows(w, sw), bias=b, dtype=torch.float32)
+    _linear_check(y, x, sx, w, sw, b)
+
+
+@gpu
+def test_linear_far_rows():
+    """Rows 8 MiB apart, whose tiles 31-bit offsets do not reach, and more outputs than one launch."""
+    m, g = _ops(), _gen(10)
+    T, N, K, ld = 700, 2 ** 22 - 5, 16, 2 ** 23 + 16
+    xs = torch.empty(T * ld, device="cuda", dtype=torch.int8)
+    x = xs.as_strided((T, K), (ld, 1))
+    x.copy_(_int8(g, T, K))
+    w = _int8(g, N, K)
+    sx, sw = _scales(g, T), _scales(g, N)
+    y = m.int8_linear(m.Int8Rows(x, sx), m.Int8Rows(w, sw))
+    for f in (slice(0, 200), slice(N // 2, N // 2 + 200), slice(N - 200, N)):
+        _linear_check(y[:, f], x, sx, w[f], sw[f], None)
+
+
+@gpu
 @pytest.mark.parametrize("T", [1, 40, 700, 3000])
 def test_linear_nan_scales_stay_in_their_row(T):
     m, g = _ops(), _gen(11)
@@ -281,6 +307,20 @@ def test_quantize_gelu(cols, xt):
     r = m.quantize_rows(x, act="gelu") # a = max |v| would be tiny)
     v = x.to(D) * torch.special.ndtr(x.to(D))
     _rows_check(r, v, 1.6e-7 * x.to(D).abs() + 4 * U * v.abs())
+
+
+@gpu
+def test_quantize_more_rows_than_one_launch():
+    """A wave per row: 2^26 rows are 2^32 threads, which no grid holds."""
+    m = _ops()
+    rows = 2 ** 26 + 77
+    x = (torch.arange(rows, device="cuda", dtype=torch.int32) % 4001 - 2000).to(torch.float16)[:, None]
+    r = m.quantize_rows(x)
+    a = x[:, 0].float()
+    assert torch.equal(r.q[:, 0].to(torch.int32), torch.sign(a).to(torch.int32) * 127)
+    assert torch.equal(r.scale, (a.to(D).abs() / 127).float())   # (no quotient is near a tie: 127 is odd)
+    v = r.dequantize(torch.float32)
+    assert torch.equal(v[:, 0], r.q[:, 0].float() * r.scale)
 
 
 @gpu
@@ -529,6 +569,15 @@ def test_two_streams_and_threads_at_once():
     for t in threads:
         t.join()
     assert not bad
+
+
+@gpu
+def test_rows_keep_their_checked_buffers():
+    m = _ops()
+    r = m.quantize_rows(torch.ones(3, 5, device="cuda"))
+    for name in ("q", "scale"):
+        with pytest.raises(AttributeError):
+            setattr(r, name, torch.ones(3))
 
 
 @gpu
