@@ -29,13 +29,16 @@ static void launch_rows(const I8RowArgs& a, hipStream_t st) {
 // The narrowest layout that holds a row.  Up to 2048 columns a wave per row (a workgroup per row
 // pays its barriers three times: 60000 x 384 LayerNorm 45 us, 89 with 4 waves a row; 65536 x 2048
 // RMS 172, 184), above that 2 chunks per thread (30000 x 8192 RMS 313 us, 349 with 4 waves x 4 chunks,
-// 416 with 16 x 1; 20000 x 16384: 449, 493 with 16 x 4).
+// 416 with 16 x 1; 20000 x 16384: 449, 493 with 16 x 4).  Idle lanes cost where arithmetic counts (GELU of
+// 65521 x 5000: 6 waves 240 us, 8 waves 281; 65521 x 2560: 3 waves 119, 4 waves 145).
 template <int MODE>
 static void launch_rows_mode(const I8RowArgs& a, hipStream_t st) {
   if (a.cols <= 512) launch_rows<MODE, 1, 1>(a, st);
   else if (a.cols <= 1024) launch_rows<MODE, 1, 2>(a, st);
   else if (a.cols <= 2048) launch_rows<MODE, 1, 4>(a, st);
+  else if (a.cols <= 3 * 1024) launch_rows<MODE, 3, 2>(a, st);
   else if (a.cols <= 4096) launch_rows<MODE, 4, 2>(a, st);
+  else if (a.cols <= 6 * 1024) launch_rows<MODE, 6, 2>(a, st);
   else if (a.cols <= 8192) launch_rows<MODE, 8, 2>(a, st);
   else if (a.cols <= 16384) launch_rows<MODE, 16, 2>(a, st);
   else launch_rows<MODE, 16, 4>(a, st);

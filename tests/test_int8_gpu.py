@@ -200,8 +200,8 @@ def test_empty_calls():
 
 
 # ---- quantise -----------------------------------------------------------------------------
-COLS = [1, 3, 7, 8, 9, 17, 64, 255, 384, 511, 512, 513, 768, 1000, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096,
-        4097, 8191, 8192, 8193, 16384, 20001, 32767, 32768]
+COLS = [1, 3, 7, 8, 9, 17, 64, 255, 384, 511, 512, 513, 768, 1000, 1023, 1024, 1025, 2047, 2048, 2049, 2999, 4095, 4096,
+        4097, 6143, 6145, 8191, 8192, 8193, 16384, 20001, 32767, 32768]
 
 
 def _quant_definition(v32):
@@ -299,7 +299,7 @@ def _rows_check(r, v, dv):
 
 @gpu
 @pytest.mark.parametrize("xt", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("cols", [1, 9, 384, 1536, 4096, 4097, 8200])
+@pytest.mark.parametrize("cols", [1, 9, 384, 1536, 2049, 2999, 4096, 4097, 6143, 6145, 8200])
 def test_quantize_gelu(cols, xt):
     m, g = _ops(), _gen(cols)
     x = (torch.randn(21, cols, generator=g, device="cuda") * 4).to(DT[xt])
@@ -405,7 +405,7 @@ def test_norm_types(xt, rt, norm):
 
 @gpu
 @pytest.mark.parametrize("norm", ["layer", "rms"])
-@pytest.mark.parametrize("cols", [40, 768, 1001, 5000])
+@pytest.mark.parametrize("cols", [40, 768, 1001, 2500, 5000, 7000])
 def test_norm_in_place_and_strided(cols, norm):
     """sum_out over the residual, norm_out over the residual or x; rows of wider buffers, aligned
     and not; what lies around the outputs stays."""
