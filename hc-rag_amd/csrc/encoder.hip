@@ -70,6 +70,7 @@ static constexpr int kEncSplits = 2;
 // (r04a measured the split slower, before the K-split remainder and with it on)
 static constexpr int kF32Streams = 2;
 static constexpr int64_t kEncSplitMinSeqs = 128;   // smaller batches run on one stream
+static constexpr int64_t kI8SplitPositions = 16384; // (HCR_I8: sequences x their padded length)
 
 struct hcr_encoder {
   int device = 0;
@@ -834,7 +835,10 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   // with the split, the f32 mode 66.2k -> 63.9k (its split GEMMs hold 128 KiB of LDS per
   // workgroup and thrash each other's weights): split by default in the fast modes only
   const int want = enc_hooks().streams > 0 ? enc_hooks().streams : (e->dtype == HCR_F32 ? kF32Streams : kEncSplits);
-  const int splits = (want <= 1 || n < kEncSplitMinSeqs) ? 1 : kEncSplits;
+  // (i8: two streams lose below that many positions -- bge-base shape, ms with 1 / 2: 256 x 32 1.88 / 1.95,
+  // 1024 x 32 5.62 / 5.55, 4096 x 32 20.3 / 20.2; MiniLM 256 x 32 0.60 / 0.73, 4096 x 32 5.4 / 5.14)
+  const bool few = n < kEncSplitMinSeqs || (e->dtype == HCR_I8 && n * S <= kI8SplitPositions && enc_hooks().streams <= 0);
+  const int splits = (want <= 1 || few) ? 1 : kEncSplits;
   for (EncWork& w : e->work) w.whole_tiles = splits > 1 && e->dtype == HCR_F32;
   if (splits == 1) return run(e->work[0], 0, n, st);
   // Sub-batches of n / splits sequences, the first on the caller's stream, the others on streams of

@@ -121,3 +121,31 @@ def test_device_call_empty_masks_and_names():
     mask[:] = 0
     assert np.array_equal(enc.encode_ids(ids, mask), np.zeros_like(want))
     assert enc.encode_ids(ids[:0], mask[:0]).shape == (0, enc.hidden)
+
+
+@pytest.mark.parametrize("dtype", ["i8", "f16"])
+def test_calls_on_two_streams_one_after_the_other(dtype):
+    """A large batch is split over two streams, one of them the caller's: the next call may come on
+    another stream without a wait in between."""
+    conf, m = _hf_model(MINILM, 6)
+    enc = _encoder(conf, m, dtype)
+    rng = np.random.default_rng(8)
+    host = [_batch(rng, 300, 64, MINILM["vocab_size"]) for _ in range(4)]
+    batches = [tuple(torch.from_numpy(a).cuda() for a in b) for b in host]
+    want = []
+    for ids, mask in batches:
+        out = torch.empty(len(ids), enc.hidden, device="cuda")
+        enc.encode_device(ids, mask, out)
+        torch.cuda.synchronize()
+        want.append(out)
+    if dtype == "i8":                             # (one sequence: one stream, kernels for few tokens)
+        assert np.array_equal(want[1][250].cpu().numpy(), enc.encode_ids(*(a[250:251] for a in host[1]))[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.full_like(w, -1.0) for w in want]
+    torch.cuda.synchronize()
+    for i, (ids, mask) in enumerate(batches):
+        with torch.cuda.stream(streams[i % 2]):
+            enc.encode_device(ids, mask, outs[i])
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
