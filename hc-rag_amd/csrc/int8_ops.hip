@@ -213,41 +213,39 @@ extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, 
   return int8_rows_launch(act == HCR_ACT_GELU ? I8_GELU : I8_QUANT, a, (hipStream_t)stream);
 }
 
-extern "C" int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, const void* d_residual,
-                                          int r_dtype, int64_t ldr, int64_t rows, int64_t cols, int norm,
-                                          const float* d_weight, const float* d_bias, float eps, void* d_sum,
-                                          int64_t ldsum, void* d_norm, int norm_dtype, int64_t ldnorm, int8_t* d_q,
-                                          int64_t ldq, float* d_scale, void* stream) {
-  CHECK(check_rows(rows, cols, kI8MaxRowCols));
-  if (norm != HCR_NORM_LAYER && norm != HCR_NORM_RMS) return hcr_set_errorf(HCR_EINVAL, "unknown norm %d", norm);
-  if (!(eps >= 0.f)) return hcr_set_error(HCR_EINVAL, "eps must be >= 0");
-  if (d_sum && !d_residual) return hcr_set_error(HCR_EINVAL, "a sum output needs a residual");
-  if (rows == 0) return HCR_OK;
-  if (!d_x || !d_weight || !d_q || !d_scale) return hcr_set_error(HCR_EINVAL, "NULL buffer");
-  CHECK(check_floats("x", d_x, x_dtype, ldx, cols));
-  if (d_residual) CHECK(check_floats("residual", d_residual, r_dtype, ldr, cols));
-  if (d_sum) CHECK(check_floats("sum", d_sum, r_dtype, ldsum, cols));
-  if (d_norm) CHECK(check_floats("norm output", d_norm, norm_dtype, ldnorm, cols));
-  CHECK(check_int8("q", d_q, ldq, cols));
-  if (!on(d_scale, 4) || !on(d_weight, 4) || !on(d_bias, 4))
+extern "C" int hcr_norm_quant_rows_device(const hcr_norm_quant_args* args, void* stream) {
+  if (!args) return hcr_set_error(HCR_EINVAL, "args is NULL");
+  const hcr_norm_quant_args& n = *args;
+  CHECK(check_rows(n.rows, n.cols, kI8MaxRowCols));
+  if (n.norm != HCR_NORM_LAYER && n.norm != HCR_NORM_RMS) return hcr_set_errorf(HCR_EINVAL, "unknown norm %d", n.norm);
+  if (!(n.eps >= 0.f)) return hcr_set_error(HCR_EINVAL, "eps must be >= 0");
+  if (n.sum && !n.residual) return hcr_set_error(HCR_EINVAL, "a sum output needs a residual");
+  if (n.rows == 0) return HCR_OK;
+  if (!n.x || !n.weight || !n.q || !n.scale) return hcr_set_error(HCR_EINVAL, "NULL buffer");
+  CHECK(check_floats("x", n.x, n.x_dtype, n.ldx, n.cols));
+  if (n.residual) CHECK(check_floats("residual", n.residual, n.residual_dtype, n.ldr, n.cols));
+  if (n.sum) CHECK(check_floats("sum", n.sum, n.residual_dtype, n.ldsum, n.cols));
+  if (n.norm_out) CHECK(check_floats("norm output", n.norm_out, n.norm_dtype, n.ldnorm, n.cols));
+  CHECK(check_int8("q", n.q, n.ldq, n.cols));
+  if (!on(n.scale, 4) || !on(n.weight, 4) || !on(n.bias, 4))
     return hcr_set_error(HCR_EINVAL, "scale, weight or bias: not aligned to its elements");
-  CHECK(check_same("the sum", d_sum, r_dtype, ldsum, "the residual", d_residual, r_dtype, ldr));
-  CHECK(check_same("the norm output", d_norm, norm_dtype, ldnorm, "x", d_x, x_dtype, ldx));
-  CHECK(check_same("the norm output", d_norm, norm_dtype, ldnorm, "the residual", d_residual, r_dtype, ldr));
-  CHECK(check_apart("the sum", d_sum, "x", d_x));
-  CHECK(check_apart("the sum", d_sum, "the norm output", d_norm));
-  CHECK(check_apart("q", d_q, "x", d_x));
-  CHECK(check_apart("q", d_q, "the residual", d_residual));
-  CHECK(check_apart("q", d_q, "the sum", d_sum));
-  CHECK(check_apart("q", d_q, "the norm output", d_norm));
+  CHECK(check_same("the sum", n.sum, n.residual_dtype, n.ldsum, "the residual", n.residual, n.residual_dtype, n.ldr));
+  CHECK(check_same("the norm output", n.norm_out, n.norm_dtype, n.ldnorm, "x", n.x, n.x_dtype, n.ldx));
+  CHECK(check_same("the norm output", n.norm_out, n.norm_dtype, n.ldnorm, "the residual", n.residual, n.residual_dtype, n.ldr));
+  CHECK(check_apart("the sum", n.sum, "x", n.x));
+  CHECK(check_apart("the sum", n.sum, "the norm output", n.norm_out));
+  CHECK(check_apart("q", n.q, "x", n.x));
+  CHECK(check_apart("q", n.q, "the residual", n.residual));
+  CHECK(check_apart("q", n.q, "the sum", n.sum));
+  CHECK(check_apart("q", n.q, "the norm output", n.norm_out));
   I8RowArgs a{};
-  a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
-  a.r = d_residual; a.ldr = ldr; a.rt = d_residual ? r_dtype : HCR_F32;
-  a.sum = d_sum; a.ldsum = ldsum;
-  a.y = d_norm; a.ldy = ldnorm; a.yt = norm_dtype;
-  a.g = d_weight; a.b = d_bias; a.eps = eps;
-  a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = (int)cols;
-  return int8_rows_launch(norm == HCR_NORM_LAYER ? I8_LAYER : I8_RMS, a, (hipStream_t)stream);
+  a.x = n.x; a.ldx = n.ldx; a.xt = n.x_dtype;
+  a.r = n.residual; a.ldr = n.ldr; a.rt = n.residual ? n.residual_dtype : HCR_F32;
+  a.sum = n.sum; a.ldsum = n.ldsum;
+  a.y = n.norm_out; a.ldy = n.ldnorm; a.yt = n.norm_dtype;
+  a.g = n.weight; a.b = n.bias; a.eps = n.eps;
+  a.q = n.q; a.ldq = n.ldq; a.scale = n.scale; a.rows = n.rows; a.cols = (int)n.cols;
+  return int8_rows_launch(n.norm == HCR_NORM_LAYER ? I8_LAYER : I8_RMS, a, (hipStream_t)stream);
 }
 
 extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows, int64_t cols,

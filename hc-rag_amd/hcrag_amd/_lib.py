@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint8, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +19,10 @@ HCR_F16, HCR_BF16, HCR_F32, HCR_I8 = 0, 1, 2, 3
 HCR_SCORE_COSINE, HCR_SCORE_UNIT = 0, 1
 HCR_ACT_NONE, HCR_ACT_GELU = 0, 1
 HCR_NORM_LAYER, HCR_NORM_RMS = 0, 1
+
+
+# hcr_norm_quant_args, in order; packed into bytes (one argument instead of 21, 0.6 us instead of 3)
+NORM_QUANT_ARGS = struct.Struct("@PqPqPPPqPqPqPqqiiiif0P")
 
 
 class HcrError(RuntimeError):
@@ -103,10 +108,7 @@ _SIGS = {
                                   c_void_p]),
     "hcr_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p,
                                       c_int64, c_void_p, c_void_p]),
-    "hcr_norm_quant_rows_device": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
-                                           c_int64, c_int64, c_int, c_void_p, c_void_p, c_float,
-                                           c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p,
-                                           c_int64, c_void_p, c_void_p]),
+    "hcr_norm_quant_rows_device": (c_int, [c_char_p, c_void_p]),     # NORM_QUANT_ARGS packed
     "hcr_dequant_rows_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                         c_int, c_int64, c_void_p]),
     "hcr_int8_linear_device": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,

@@ -21,7 +21,7 @@ from typing import Optional
 import torch
 
 from ._lib import (HCR_ACT_GELU, HCR_ACT_NONE, HCR_BF16, HCR_F16, HCR_F32, HCR_NORM_LAYER,
-                   HCR_NORM_RMS, check, lib)
+                   HCR_NORM_RMS, NORM_QUANT_ARGS, check, lib)
 
 _DTYPE = {torch.float16: HCR_F16, torch.bfloat16: HCR_BF16, torch.float32: HCR_F32}
 _ACT = {"none": HCR_ACT_NONE, "gelu": HCR_ACT_GELU}
@@ -31,6 +31,7 @@ _grad_on = torch.is_grad_enabled
 _current_device = torch._C._cuda_getDevice            # (torch.cuda.current_device without its init check:
 _current_stream = torch._C._cuda_getCurrentRawStream  # the operands are device tensors; 0.1 us against 1.4)
 _new = object.__new__
+_pack_norm = NORM_QUANT_ARGS.pack
 
 
 # A single token's call is bound by what the host does, so the checks are one expression per
@@ -192,7 +193,7 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         _refuse(weight, "weight", (_F32,), 1, device)
     if weight.shape[0] != cols:
         raise ValueError(f"weight: {weight.shape[0]} elements, expected {cols}")
-    bias_p = resid_p = sum_p = norm_p = None
+    bias_p = resid_p = sum_p = norm_p = 0
     resid_t = norm_t = HCR_F32
     resid_ld = sum_ld = norm_ld = 0
     if bias is not None:
@@ -213,9 +214,10 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         norm_t, norm_ld = _rows_operand(norm_out, "norm_out", shape, device)
         norm_p = norm_out.data_ptr()
     out = _int8_out(out, rows, cols, x)
-    _norm_quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), resid_p, resid_t, resid_ld, rows, cols, _NORM[norm],
-                weight.data_ptr(), bias_p, eps, sum_p, sum_ld, norm_p, norm_t, norm_ld, out._q.data_ptr(), _ld(out._q),
-                out._scale.data_ptr())
+    q = out._q
+    _norm_quant(device, _pack_norm(x.data_ptr(), _ld(x), resid_p, resid_ld, weight.data_ptr(), bias_p, sum_p, sum_ld,
+                                   norm_p, norm_ld, q.data_ptr(), _ld(q), out._scale.data_ptr(), rows, cols,
+                                   _DTYPE[x.dtype], resid_t, norm_t, _NORM[norm], eps))
     return out
 
 

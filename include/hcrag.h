@@ -377,15 +377,24 @@ int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t row
 
 /* h = x + residual (residual NULL: h = x); v = norm(h) * weight + bias (bias NULL: 0), with
  * norm(h) = (h - mean) / sqrt(var + eps) (HCR_NORM_LAYER) or h / sqrt(mean(h^2) + eps)
- * (HCR_NORM_RMS), all in fp32; int8 rows of v.  d_sum (NULL: not stored) receives h in the
- * residual's type, d_norm (NULL: not stored) v in norm_dtype.  d_sum may be the residual itself and
- * d_norm x or the residual itself (same type and stride); other buffers must not overlap.  weight
- * and bias: fp32, cols elements. */
-int hcr_norm_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, const void* d_residual,
-                               int r_dtype, int64_t ldr, int64_t rows, int64_t cols, int norm,
-                               const float* d_weight, const float* d_bias, float eps, void* d_sum,
-                               int64_t ldsum, void* d_norm, int norm_dtype, int64_t ldnorm,
-                               int8_t* d_q, int64_t ldq, float* d_scale, void* stream);
+ * (HCR_NORM_RMS), all in fp32; int8 rows of v.  sum (NULL: not stored) receives h in the
+ * residual's type, norm_out (NULL: not stored) v in norm_dtype.  sum may be the residual itself and
+ * norm_out x or the residual itself (same type and stride); other buffers must not overlap. */
+typedef struct {
+  const void* x;        int64_t ldx;      /* [rows][cols] of x_dtype */
+  const void* residual; int64_t ldr;      /* [rows][cols] of residual_dtype, or NULL */
+  const float* weight;                    /* [cols] */
+  const float* bias;                      /* [cols], or NULL */
+  void* sum;            int64_t ldsum;    /* [rows][cols] of residual_dtype, or NULL */
+  void* norm_out;       int64_t ldnorm;   /* [rows][cols] of norm_dtype, or NULL */
+  int8_t* q;            int64_t ldq;
+  float* scale;
+  int64_t rows, cols;
+  int32_t x_dtype, residual_dtype, norm_dtype;
+  int32_t norm;                           /* hcr_norm */
+  float eps;
+} hcr_norm_quant_args;
+int hcr_norm_quant_rows_device(const hcr_norm_quant_args* args, void* stream);
 
 /* out [rows][cols] = q * scale, rounded to out_dtype (1 <= cols <= 131071). */
 int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const float* d_scale, int64_t rows,

@@ -16,8 +16,9 @@ def quant(x=P, xt=F16, ldx=64, rows=4, cols=64, act=0, q=P, ldq=64, scale=P):
 
 def norm(x=P, xt=F16, ldx=64, r=P, rt=F32, ldr=64, rows=4, cols=64, kind=0, w=P, b=P, eps=1e-6, s=P,
          lds=64, y=P, yt=F16, ldy=64, q=P, ldq=64, scale=P):
-    return _lib.lib().hcr_norm_quant_rows_device(x, xt, ldx, r, rt, ldr, rows, cols, kind, w, b, eps, s, lds,
-                                                 y, yt, ldy, q, ldq, scale, None)
+    args = _lib.NORM_QUANT_ARGS.pack(x or 0, ldx, r or 0, ldr, w or 0, b or 0, s or 0, lds, y or 0, ldy, q or 0, ldq,
+                                     scale or 0, rows, cols, xt, rt, yt, kind, eps)
+    return _lib.lib().hcr_norm_quant_rows_device(args, None)
 
 
 def dequant(q=P, ldq=64, scale=P, rows=4, cols=64, out=P, ot=F16, ldo=64):
@@ -76,6 +77,22 @@ def test_sizes_past_32_bits_are_refused_not_cut(call, name):
     strides = {quant: ("ldx", "ldq"), norm: ("ldx", "ldr", "lds", "ldy", "ldq"), dequant: ("ldq", "ldo"),
                linear: ("ldx", "ldw", "ldo")}[call]
     assert call(**{**OWN[call], name: (1 << 32) + 8, **{k: far for k in strides}}) == _lib.HCR_EINVAL
+
+
+def test_packed_arguments_are_the_struct():
+    import ctypes
+
+    class Args(ctypes.Structure):                 # hcr_norm_quant_args, include/hcrag.h
+        _fields_ = [(n, ctypes.c_void_p if n in ("x", "r", "w", "b", "s", "y", "q", "scale") else ctypes.c_int64)
+                    for n in "x ldx r ldr w b s lds y ldy q ldq scale rows cols".split()] + [
+            (n, ctypes.c_int32) for n in ("xt", "rt", "yt", "kind")] + [("eps", ctypes.c_float)]
+
+    values = [*range(1, 16), 1, 2, 0, 1, 0.5]
+    packed = _lib.NORM_QUANT_ARGS.pack(*values)
+    assert len(packed) == ctypes.sizeof(Args)
+    a = Args.from_buffer_copy(packed)
+    assert [getattr(a, n) for n, _ in Args._fields_] == values
+    assert _lib.lib().hcr_norm_quant_rows_device(None, None) == _lib.HCR_EINVAL
 
 
 def test_nothing_to_do_is_ok():
