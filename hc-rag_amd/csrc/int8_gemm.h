@@ -145,7 +145,8 @@ __host__ __device__ constexpr int i8_size(int ot) { return ot == HCR_F32 ? 4 : 2
 // sw, sb, sx: LDS addresses of the wave's w scales, biases and x scales.
 // Measured against staging the tile through LDS for 256-byte stores, with 128 x 256 tiles of 4 waves
 // at K = 768, N = 2304, T = 21853: 60.8 us, staged 62.8.
-template <int OT, int MT, bool ODD>
+// NT: the stores are non-temporal (a result that no cache holds).
+template <int OT, int MT, bool ODD, bool NT>
 __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_buffer_rsrc_t o_rsrc,
                                               const intx4 (&acc)[MT][4], int lane, int f0, int t0, uint32_t sw,
                                               uint32_t sb, uint32_t sx) {
@@ -199,7 +200,7 @@ __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_bu
       }
 #pragma unroll
       for (int j = 0; j < NU; ++j) {
-        __builtin_amdgcn_raw_buffer_store_b128(u[j], o_rsrc, f[j] + PER <= left ? row[n] + f[j] * ES : I8_FAR, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(u[j], o_rsrc, f[j] + PER <= left ? row[n] + f[j] * ES : I8_FAR, 0, NT ? 2 : 0);
         if (ODD && left < 16 * MT) {                   // (uniform: the wave holds the row's last features)
           const uint32_t w[4] = {u[j][0], u[j][1], u[j][2], u[j][3]};
 #pragma unroll
@@ -216,7 +217,7 @@ __device__ __forceinline__ void i8_store_tile(const I8LinearArgs& a, __amdgpu_bu
 
 // A workgroup of WM x WN waves per tile of 16 MT WM features x 64 WN tokens; OCC waves per SIMD, so that
 // while one workgroup of a CU waits for its stage or stores its tile another multiplies.
-template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC>
+template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC, bool NT>
 __global__ void __launch_bounds__(64 * WM * WN, OCC)
 int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
   constexpr int KB = 64, FT = 16 * MT * WM, TT = 64 * WN, NW = WM * WN;
@@ -312,7 +313,7 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the ring's last pieces, before the LDS is given back
   const __amdgpu_buffer_rsrc_t o_rsrc = __builtin_amdgcn_make_buffer_rsrc(
       uniform_ptr(a.out), (short)0, __builtin_amdgcn_readfirstlane(((a.T - 1) * (int)a.ldo + a.N) * i8_size(OT)), 0x00020000);
-  i8_store_tile<OT, MT, ODD>(a, o_rsrc, acc, lane, f0 + wm * 16 * MT, t0 + wn * 64, lds_addr(sc + wm * 16 * MT),
+  i8_store_tile<OT, MT, ODD, NT>(a, o_rsrc, acc, lane, f0 + wm * 16 * MT, t0 + wn * 64, lds_addr(sc + wm * 16 * MT),
                              lds_addr(sc + FT + wm * 16 * MT), lds_addr(sc + 2 * FT + wn * 64));
 }
 
@@ -335,7 +336,7 @@ int8_linear_tiles(I8LinearArgs a, int n_tiles_feat) {
 //     4 stages ahead of group 1's epilogue: at 2 stages a tile, 2 tiles).
 // Host-checked: K > 64 (2 stages a tile at least).
 // OT: hcr_dtype of out
-template <int OT, bool ODD>
+template <int OT, bool ODD, bool NT>
 __global__ void __launch_bounds__(512, 2)
 int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
   constexpr int KB = 64, NST = 4, FT = 256, TT = 256, A_BYTES = FT * KB, STAGE = (FT + TT) * KB;
@@ -415,7 +416,7 @@ int8_linear_stream(I8LinearArgs a, int n_tiles_feat, unsigned n_tiles) {
     int f0, t0;
     tile_at(i, f0, t0);
     const uint32_t s0 = lds_addr(sc[i & 3]);
-    i8_store_tile<OT, 8, ODD>(a, o_rsrc, acc, lane, f0 + wm * 128, t0 + wn * 64, s0 + wm * 512,
+    i8_store_tile<OT, 8, ODD, NT>(a, o_rsrc, acc, lane, f0 + wm * 128, t0 + wn * 64, s0 + wm * 512,
                               s0 + (FT + wm * 128) * 4, s0 + (2 * FT + wn * 64) * 4);
   };
 

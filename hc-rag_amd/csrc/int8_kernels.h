@@ -27,8 +27,8 @@ typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 // finite value, and such a row gets scale NaN and q = 0, so that a product with it is NaN.  A row
 // below 2^-100 counts as zeros (scale 0, q 0): 127 / a would leave fp32's range.
 // Bound by memory (MI355X; a copy of 8 GiB moves 4.6 TB/s): RMS norm with residual of 65521 x 4096 bf16
-// 1.88 GB in 338-360 us, LayerNorm of 32749 x 768 (f16 + f32 -> f32) 52 us (5.3 TB/s), quantisation of
-// 65521 x 4096 f16 138 us (5.8 TB/s), with GELU 160 us, where arithmetic and memory meet.
+// 1.88 GB in 345 us (5.4 TB/s), LayerNorm of 32749 x 768 (f16 + f32 -> f32) 52 us (5.3 TB/s), quantisation
+// of 65521 x 4096 f16 118 us (6.8 TB/s), with GELU 158 us, where arithmetic and memory meet.
 // -------------------------------------------------------------------------------------
 
 // gelu(x) = x Phi(x) = x / (1 + 2^-z), z = log2(Phi / (1 - Phi)) = x g(x^2): g as a polynomial fitted so
@@ -59,18 +59,29 @@ __device__ __forceinline__ uint32_t i8_step(float v, float inv) {
 // 16 bytes at any alignment: one instruction, the hardware takes unaligned vectors (rows of odd
 // widths, 65521 x 1531 bf16: 139 us element by element).
 typedef uint32_t uintx4_any __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ uintx4 i8_load16(const char* p) { return *reinterpret_cast<const uintx4_any*>(p); }
-__device__ __forceinline__ void i8_store16(char* p, uintx4 u) { *reinterpret_cast<uintx4_any*>(p) = u; }
+// NT: not to be kept in the caches (non-temporal).
+template <bool NT = false>
+__device__ __forceinline__ uintx4 i8_load16(const char* p) {
+  const uintx4_any* v = reinterpret_cast<const uintx4_any*>(p);
+  if constexpr (NT) return __builtin_nontemporal_load(v);
+  else return *v;
+}
+template <bool NT = false>
+__device__ __forceinline__ void i8_store16(char* p, uintx4 u) {
+  uintx4_any* v = reinterpret_cast<uintx4_any*>(p);
+  if constexpr (NT) __builtin_nontemporal_store((uintx4_any)u, v);
+  else *v = u;
+}
 
 struct I8Raw { uintx4 a, b; };     // 8 elements as loaded: 16-bit types in a, f32 in a and b
 
 // elements [i, i + 8) of a row of cols: whole chunks as vectors, the row's last, partial one element
 // by element (the row's last element again past its end: the caller drops those)
-template <bool F32>
+template <bool F32, bool NT = false>
 __device__ __forceinline__ void i8_load(I8Raw& o, const char* row, int i, int cols) {
   if (i + 8 <= cols) {
     const char* p = row + (int64_t)i * (F32 ? 4 : 2);
-    o.a = i8_load16(p);
+    o.a = i8_load16<NT>(p);
     if constexpr (F32) o.b = i8_load16(p + 16);
   } else if (i < cols) {
     uint32_t w[8];
@@ -114,6 +125,7 @@ __device__ __forceinline__ uint32_t i8_pack2(float x, float y) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{x, y}), T2));
 }
 // elements [i, i + 8) of a row of cols, those that exist
+template <bool NT>
 __device__ __forceinline__ void i8_store(char* row, int type, int i, int cols, const float (&v)[8]) {
   if (type == HCR_F32) {
     char* p = row + (int64_t)i * 4;
@@ -131,7 +143,7 @@ __device__ __forceinline__ void i8_store(char* row, int type, int i, int cols, c
   else h = uintx4{i8_pack2<_Float16>(v[0], v[1]), i8_pack2<_Float16>(v[2], v[3]), i8_pack2<_Float16>(v[4], v[5]), i8_pack2<_Float16>(v[6], v[7])};
   char* p = row + (int64_t)i * 2;
   if (i + 8 <= cols) {
-    i8_store16(p, h);
+    i8_store16<NT>(p, h);
   } else {
 #pragma unroll
     for (int e = 0; e < 7; ++e)
@@ -177,7 +189,10 @@ __device__ __forceinline__ float i8_row_sum(float s, uint32_t* red, int wave, in
 }
 
 // One row per WAVES waves; WAVES == 1 puts 4 rows in a workgroup.  Covers cols <= 512 WAVES NCH.
-template <int MODE, int WAVES, int NCH>
+// NT: x, the residual and what is stored pass by the caches (but f32 rows, of which a lane takes two
+// vectors, each half of its lines, and the int8 rows of a mere quantisation: 65521 x 4096 f16 118 us, with
+// them 125).
+template <int MODE, int WAVES, int NCH, bool NT>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 rows_to_int8_kernel(I8RowArgs a) {
   __shared__ uint32_t red[WAVES > 1 ? WAVES : 1];
@@ -198,7 +213,7 @@ rows_to_int8_kernel(I8RowArgs a) {
     for (int c = 0; c < NCH; ++c) i8_load<true>(xs[c], xr, (tid + NTH * c) * 8, a.cols);
   } else {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) i8_load<false>(xs[c], xr, (tid + NTH * c) * 8, a.cols);
+    for (int c = 0; c < NCH; ++c) i8_load<false, NT>(xs[c], xr, (tid + NTH * c) * 8, a.cols);
   }
   if constexpr (NORM) {
     if (a.r) {
@@ -207,7 +222,7 @@ rows_to_int8_kernel(I8RowArgs a) {
         for (int c = 0; c < NCH; ++c) i8_load<true>(rs[c], rr, (tid + NTH * c) * 8, a.cols);
       } else {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) i8_load<false>(rs[c], rr, (tid + NTH * c) * 8, a.cols);
+        for (int c = 0; c < NCH; ++c) i8_load<false, NT>(rs[c], rr, (tid + NTH * c) * 8, a.cols);
       }
     }
   }
@@ -265,7 +280,7 @@ rows_to_int8_kernel(I8RowArgs a) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int i = (tid + NTH * c) * 8;
-        if (i < a.cols) i8_store(sr, a.rt, i, a.cols, v[c]);
+        if (i < a.cols) i8_store<NT>(sr, a.rt, i, a.cols, v[c]);
       }
     }
 #pragma unroll
@@ -292,7 +307,7 @@ rows_to_int8_kernel(I8RowArgs a) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int i = (tid + NTH * c) * 8;
-        if (i < a.cols) i8_store(yr, a.yt, i, a.cols, v[c]);
+        if (i < a.cols) i8_store<NT>(yr, a.yt, i, a.cols, v[c]);
       }
     }
   }
@@ -333,8 +348,12 @@ rows_to_int8_kernel(I8RowArgs a) {
       const uint32_t hi = __builtin_amdgcn_perm(u[4 * d + 3], u[4 * d + 2], 0x0C0C0400u);
       w[d] = zero ? 0u : lo | hi << 16;
     }
-    if (n >= 8) *reinterpret_cast<uint2*>(qr + i) = uint2{w[0], w[1]};   // (q rows start on 16 bytes)
-    else
+    if (n >= 8) {                  // (q rows start on 16 bytes)
+      typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+      uintx2* p = reinterpret_cast<uintx2*>(qr + i);
+      if constexpr (NT && NORM) __builtin_nontemporal_store(uintx2{w[0], w[1]}, p);
+      else *p = uintx2{w[0], w[1]};
+    } else
 #pragma unroll
       for (int e = 0; e < 7; ++e) if (e < n) qr[i + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
   }
@@ -342,6 +361,7 @@ rows_to_int8_kernel(I8RowArgs a) {
 
 // out = q * scale, rounded once to the output's type.  One thread per 8 elements; the last 8 of a row
 // that is no multiple of 8 overlap the ones before (the same values are stored twice).
+template <bool NT>
 __global__ void __launch_bounds__(256)
 int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, unsigned rows,
                     int cols, void* __restrict__ out, int ot, int64_t ldo) {
@@ -362,7 +382,7 @@ int8_to_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __re
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)qr[min(e, cols - 1)] * s;
   }
-  i8_store(orow, ot, i, cols, v);
+  i8_store<NT>(orow, ot, i, cols, v);
 }
 
 // -------------------------------------------------------------------------------------

@@ -12,19 +12,33 @@ using namespace hcr;
 
 namespace hcr {
 
+// What a call reads or writes beyond the 256 MiB of the memory-side cache is evicted before its next
+// use, so it goes past the caches (quantisation of 65521 x 4096 f16 138 us, so 118; dequantisation
+// 139, 118; RMS norm 360, 345).  Below that the next kernel pays more than this one gains: 65521 x 768
+// f16, dequantisation and an addition 70 us, 77 so; quantisation and a product 70, 76.
+constexpr int64_t kNtBytes = (int64_t)256 << 20;
+
 constexpr int64_t kLaunchThreads = (int64_t)1 << 31;   // per launch; a grid of 2^32 threads is refused
 
-template <int MODE, int WAVES, int NCH>
-static void launch_rows(const I8RowArgs& a, hipStream_t st) {
+template <int MODE, int WAVES, int NCH, bool NT>
+static void launch_rows_nt(const I8RowArgs& a, hipStream_t st) {
   constexpr int64_t most = kLaunchThreads / (64 * WAVES);        // rows per launch
   for (int64_t r = 0; r < a.rows; r += most) {
     I8RowArgs c = a;
     c.row0 = r;
     c.rows = std::min(most, a.rows - r);
     const unsigned grid = WAVES == 1 ? (unsigned)((c.rows + 3) / 4) : (unsigned)c.rows;
-    hipLaunchKernelGGL((rows_to_int8_kernel<MODE, WAVES, NCH>), dim3(grid), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0,
+    hipLaunchKernelGGL((rows_to_int8_kernel<MODE, WAVES, NCH, NT>), dim3(grid), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0,
                        st, c);
   }
+}
+template <int MODE, int WAVES, int NCH>
+static void launch_rows(const I8RowArgs& a, hipStream_t st) {
+  const int64_t n = a.rows * a.cols;
+  const int64_t in = n * (i8_size(a.xt) + (a.r ? i8_size(a.rt) : 0));
+  const int64_t out = n * (1 + (a.sum ? i8_size(a.rt) : 0) + (a.y ? i8_size(a.yt) : 0));
+  if (std::max(in, out) >= kNtBytes) launch_rows_nt<MODE, WAVES, NCH, true>(a, st);
+  else launch_rows_nt<MODE, WAVES, NCH, false>(a, st);
 }
 // The narrowest layout that holds a row.  Up to 2048 columns a wave per row (a workgroup per row
 // pays its barriers three times: 60000 x 384 LayerNorm 45 us, 89 with 4 waves a row; 65536 x 2048
@@ -63,12 +77,16 @@ static int launch_direct(const I8LinearArgs& a, hipStream_t st) {
 static int64_t tiles_of(const I8LinearArgs& a, int features, int tokens) {
   return (int64_t)((a.N + features - 1) / features) * ((a.T + tokens - 1) / tokens);
 }
-template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC>
+template <int OT, bool ODD, int MT, int WM, int WN, int NST, int OCC, bool NT = false>
 static void launch_tile(const I8LinearArgs& a, hipStream_t st) {
   constexpr int FT = 16 * MT * WM, TT = 64 * WN;
-  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD, MT, WM, WN, NST, OCC>), dim3((unsigned)tiles_of(a, FT, TT)),
+  hipLaunchKernelGGL((int8_linear_tiles<OT, ODD, MT, WM, WN, NST, OCC, NT>), dim3((unsigned)tiles_of(a, FT, TT)),
                      dim3(64 * WM * WN), 0, st, a, (a.N + FT - 1) / FT);
 }
+// Results of kNtBytes and more (T = 65536, K = 1024, N = 4096, f16, 512 MiB: 321 us, so 292; T = 24576, 192 MiB:
+// 112, 115), unless rows are no whole number of 16 bytes (T = 30001, K = 777, N = 2051, f32: 127, 268).
+static bool nt_out(const I8LinearArgs& a) { return (int64_t)a.T * a.N * i8_size(a.ot) >= kNtBytes; }
+
 // The widest tile that leaves every CU one, down to 64 x 128 (features x tokens; us on MI355X):
 //   64 x 128   4 waves of 32 x 64: a round takes 2.75 + 0.235 per 64 of depth (T = 2000, N = 1024, K = 4096:
 //              18.5, 128 x 128 22.8, 128 x 256 31.1; T = 4000: 30.3, 24.0, 31.7; T = 1000, N = 768, K = 768:
@@ -81,13 +99,16 @@ template <int OT, bool ODD>
 static void launch_tiles(const I8LinearArgs& a, hipStream_t st) {
   if (tiles_of(a, 64, 128) <= 256) launch_tile<OT, ODD, 2, 2, 2, 4, 3>(a, st);
   else if (tiles_of(a, 128, 128) <= 256) launch_tile<OT, ODD, 2, 4, 2, 4, 4>(a, st);
+  else if (!ODD && nt_out(a)) launch_tile<OT, ODD, 4, 2, 4, 3, 4, !ODD>(a, st);
   else launch_tile<OT, ODD, 4, 2, 4, 3, 4>(a, st);
 }
 template <int OT, bool ODD>
 static void launch_stream(const I8LinearArgs& a, hipStream_t st) {
   const int nft = (a.N + 255) / 256;
   const unsigned tiles = (unsigned)nft * ((a.T + 255) / 256);
-  hipLaunchKernelGGL((int8_linear_stream<OT, ODD>), dim3(std::min((tiles + 7) & ~7u, 256u)), dim3(512), 0, st, a, nft, tiles);
+  const dim3 grid(std::min((tiles + 7) & ~7u, 256u));
+  if (!ODD && nt_out(a)) hipLaunchKernelGGL((int8_linear_stream<OT, ODD, !ODD>), grid, dim3(512), 0, st, a, nft, tiles);
+  else hipLaunchKernelGGL((int8_linear_stream<OT, ODD, false>), grid, dim3(512), 0, st, a, nft, tiles);
 }
 template <int OT>
 static void launch_linear(const I8LinearArgs& a, bool stream, hipStream_t st) {
@@ -261,7 +282,8 @@ extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const flo
   const int64_t per = (cols + 7) / 8, most = kLaunchThreads / per;   // threads per row, rows per launch
   for (int64_t r = 0; r < rows; r += most) {
     const int64_t n = std::min(most, rows - r);
-    hipLaunchKernelGGL(int8_to_rows_kernel, dim3((unsigned)((n * per + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+    auto kernel = rows * cols * (int64_t)float_size(out_dtype) >= kNtBytes ? int8_to_rows_kernel<true> : int8_to_rows_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((n * per + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
                        d_q + r * ldq, ldq, d_scale + r, (unsigned)n, (int)cols,
                        static_cast<char*>(d_out) + r * ldo * (int64_t)float_size(out_dtype), out_dtype, ldo);
     HIPC(hipGetLastError());

@@ -571,6 +571,51 @@ def test_two_streams_and_threads_at_once():
     assert not bad
 
 
+# ---- results larger than any cache (256 MiB and more: non-temporal loads and stores) ----------
+PARTS = (slice(0, 300), slice(35000, 35300), slice(-301, None))
+
+
+@gpu
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("K", [384, 1024])
+def test_linear_past_the_caches(K, out):
+    """The same bits as parts of the batch, which the caches hold."""
+    m, g = _ops(), _gen(K)
+    T, N = 70001, 2048
+    x, w = _int8(g, T, K), _int8(g, N, K)
+    sx, sw, b = _scales(g, T), _scales(g, N), torch.randn(N, generator=g, device="cuda")
+    rows = m.Int8Rows(w, sw)
+    y = m.int8_linear(m.Int8Rows(x, sx), rows, bias=b, dtype=DT[out])
+    for p in PARTS:
+        want = m.int8_linear(m.Int8Rows(x[p], sx[p]), rows, bias=b, dtype=DT[out])
+        assert torch.equal(y[p], want)
+        _linear_check(want, x[p], sx[p], w, sw, b)
+
+
+@gpu
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("xt,rt,yt", [("bf16", "bf16", "bf16"), ("f16", "f32", "f16"), ("f32", "f16", "f32")])
+@pytest.mark.parametrize("cols", [1001, 2304])
+def test_rows_past_the_caches(cols, xt, rt, yt, norm):
+    m, g = _ops(), _gen(cols)
+    T = 70001
+    x = torch.randn(T, cols, generator=g, device="cuda").to(DT[xt])
+    r = torch.randn(T, cols, generator=g, device="cuda").to(DT[rt])
+    w, b = torch.randn(cols, generator=g, device="cuda"), torch.randn(cols, generator=g, device="cuda")
+    total, y = torch.empty_like(r), torch.empty(T, cols, device="cuda", dtype=DT[yt])
+    q = m.norm_quantize(x, w, b, residual=r, norm=norm, sum_out=total, norm_out=y)
+    gelu, v = m.quantize_rows(x, act="gelu"), q.dequantize(DT[yt])
+    for p in PARTS:
+        n = len(x[p])
+        part_total, part_y = torch.empty(n, cols, device="cuda", dtype=DT[rt]), torch.empty(n, cols, device="cuda", dtype=DT[yt])
+        part = m.norm_quantize(x[p], w, b, residual=r[p], norm=norm, sum_out=part_total, norm_out=part_y)
+        assert torch.equal(q.q[p], part.q) and torch.equal(q.scale[p], part.scale)
+        assert torch.equal(total[p], part_total) and torch.equal(y[p], part_y)
+        assert torch.equal(v[p], part.dequantize(DT[yt]))
+        part = m.quantize_rows(x[p], act="gelu")
+        assert torch.equal(gelu.q[p], part.q) and torch.equal(gelu.scale[p], part.scale)
+
+
 @gpu
 def test_rows_keep_their_checked_buffers():
     m = _ops()
