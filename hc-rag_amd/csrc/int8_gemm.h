@@ -25,11 +25,11 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
       "ds_read_b128 %0, %8\n\t"
       "ds_read_b128 %1, %8 offset:1024\n\t"
       "ds_read_b128 %2, %8 offset:2048\n\t"
-      "ds_read_b128 %3, %8 offset:3072\n\t"
+      "ds_read_b128 %3, %8 offset:0xc00\n\t"
       "ds_read_b128 %4, %9\n\t"
       "ds_read_b128 %5, %9 offset:1024\n\t"
       "ds_read_b128 %6, %9 offset:2048\n\t"
-      "ds_read_b128 %7, %9 offset:3072\n\t"
+      "ds_read_b128 %7, %9 offset:0xc00\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(av[0]), "=&v"(av[1]), "=&v"(av[2]), "=&v"(av[3]), "=&v"(bq[0]), "=&v"(bq[1]), "=&v"(bq[2]),
         "=&v"(bq[3])
@@ -44,7 +44,7 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
       "ds_read_b128 %2, %7\n\t"
       "ds_read_b128 %3, %7 offset:1024\n\t"
       "ds_read_b128 %4, %7 offset:2048\n\t"
-      "ds_read_b128 %5, %7 offset:3072\n\t"
+      "ds_read_b128 %5, %7 offset:0xc00\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(av[0]), "=&v"(av[1]), "=&v"(bq[0]), "=&v"(bq[1]), "=&v"(bq[2]), "=&v"(bq[3])
       : "v"(a), "v"(b)
@@ -67,11 +67,11 @@ __device__ __forceinline__ void i8_read_frags(uint32_t a, uint32_t b, intx4 (&av
       "ds_read_b128 %8, %[b]\n\t"
       "ds_read_b128 %9, %[b] offset:1024\n\t"
       "ds_read_b128 %10, %[b] offset:2048\n\t"
-      "ds_read_b128 %11, %[b] offset:3072\n\t"
+      "ds_read_b128 %11, %[b] offset:0xc00\n\t"
       "ds_read_b128 %0, %[a]\n\t"
       "ds_read_b128 %1, %[a] offset:1024\n\t"
       "ds_read_b128 %2, %[a] offset:2048\n\t"
-      "ds_read_b128 %3, %[a] offset:3072\n\t"
+      "ds_read_b128 %3, %[a] offset:0xc00\n\t"
       "ds_read_b128 %4, %[a] offset:4096\n\t"
       "ds_read_b128 %5, %[a] offset:5120\n\t"
       "ds_read_b128 %6, %[a] offset:6144\n\t"
