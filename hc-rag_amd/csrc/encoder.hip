@@ -840,7 +840,14 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   const bool few = n < kEncSplitMinSeqs || (e->dtype == HCR_I8 && n * S <= kI8SplitPositions && enc_hooks().streams <= 0);
   const int splits = (want <= 1 || few) ? 1 : kEncSplits;
   for (EncWork& w : e->work) w.whole_tiles = splits > 1 && e->dtype == HCR_F32;
-  if (splits == 1) return run(e->work[0], 0, n, st);
+  // (the last call may have used the first sub-batch's buffers on another stream)
+  if (!e->work[0].done) HIPC(hipEventCreateWithFlags(&e->work[0].done, hipEventDisableTiming));
+  HIPC(hipStreamWaitEvent(st, e->work[0].done, 0));
+  if (splits == 1) {
+    CHECK(run(e->work[0], 0, n, st));
+    HIPC(hipEventRecord(e->work[0].done, st));
+    return HCR_OK;
+  }
   // Sub-batches of n / splits sequences, the first on the caller's stream, the others on streams of
   // their own (ordered after the caller's work through ev_in; the caller's stream waits for their
   // `done` events): every
@@ -852,15 +859,14 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   for (int i = 0; i < splits; ++i) {
     EncWork& w = e->work[i];
     const int64_t s0 = n * i / splits, s1 = n * (i + 1) / splits;
-    if (!w.done) HIPC(hipEventCreateWithFlags(&w.done, hipEventDisableTiming));
     if (i == 0) {
-      HIPC(hipStreamWaitEvent(st, w.done, 0));          // (the last call's stream may be another)
       CHECK(run(w, s0, s1 - s0, st));
       HIPC(hipEventRecord(w.done, st));
       continue;
     }
     // default priority: work on streams of different priorities has hung MI355X boards
     if (!w.st) HIPC(hipStreamCreateWithFlags(&w.st, hipStreamNonBlocking));
+    if (!w.done) HIPC(hipEventCreateWithFlags(&w.done, hipEventDisableTiming));
     HIPC(hipStreamWaitEvent(w.st, e->ev_in, 0));
     CHECK(run(w, s0, s1 - s0, w.st));
     HIPC(hipEventRecord(w.done, w.st));
