@@ -95,6 +95,16 @@ def _device(t, name: str, dtypes, dim: int) -> int:
     return device
 
 
+def _rows_device(r: "Int8Rows", name: str) -> int:
+    """The device index of int8 rows, which a loader may have restored to the host."""
+    device = r._q.get_device()
+    if device < 0:
+        _refuse(r._q, name, (_I8,), 2)
+    if r._scale.get_device() != device:
+        _refuse(r._scale, name + ".scale", (_F32,), 1, device)
+    return device
+
+
 def _ld(t) -> int:
     """Row stride in elements; of at most one row, any that its width allows."""
     rows, cols = t.shape
@@ -124,10 +134,11 @@ class Int8Rows:
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Int8Rows":
-        """Uninitialised rows, laid out as the operators want them."""
+        """Uninitialised rows on a GPU, laid out as the operators want them."""
         self = _new(cls)
         self._q = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=_I8, device=device)
         self._scale = torch.empty(rows, dtype=_F32, device=device)
+        _rows_device(self, "rows")
         return self
 
     @property
@@ -142,11 +153,12 @@ class Int8Rows:
         """[rows, cols] of the values that the rows stand for, rounded to ``dtype``."""
         if dtype not in _DTYPE:
             raise ValueError(f"dtype {dtype} is not supported here")
+        device = _rows_device(self, "rows")
         q = self._q
         rows, cols = q.shape
         out = q.new_empty((rows, cols), dtype=dtype)
         if rows:
-            _dequant(q.get_device(), q.data_ptr(), _ld(q), self._scale.data_ptr(), rows, cols, out.data_ptr(),
+            _dequant(device, q.data_ptr(), _ld(q), self._scale.data_ptr(), rows, cols, out.data_ptr(),
                      _DTYPE[dtype], cols)
         return out
 
@@ -154,7 +166,7 @@ class Int8Rows:
 def _int8_out(out: Optional[Int8Rows], rows: int, cols: int, like: torch.Tensor) -> Int8Rows:
     if out is None:
         return Int8Rows.empty(rows, cols, like.device)
-    if tuple(out._q.shape) != (rows, cols) or out._q.device != like.device:
+    if tuple(out._q.shape) != (rows, cols) or _rows_device(out, "out") != like.get_device():
         raise ValueError(f"out: {tuple(out._q.shape)} on {out._q.device}, expected {(rows, cols)} on {like.device}")
     return out
 
@@ -239,10 +251,10 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
     xq, wq = x._q, w._q
     rows, depth = xq.shape
     features, depth_w = wq.shape
-    device = xq.get_device()
+    device = _rows_device(x, "x")
     if depth_w != depth:
         raise ValueError(f"x has depth {depth}, w {depth_w}")
-    if wq.get_device() != device:
+    if _rows_device(w, "w") != device:
         raise ValueError(f"w: on {wq.device}, x on {xq.device}")
     bias_p = None
     if bias is not None:
