@@ -8,7 +8,8 @@ rows) are the pieces that ``BertEncoder(dtype="i8")`` runs its layers on; they b
 
 Every call is enqueued on torch's current stream of the tensors' device and returns at once;
 calls can be captured into graphs.  They compute no gradients: a tensor that asks for one is
-refused while gradients are recorded.  No CPU fallback: without the HIP library they raise.
+refused while gradients are recorded, and what a call writes into (``out``, ``sum_out``, ``norm_out``)
+counts as modified in place.  No CPU fallback: without the HIP library they raise.
 
     w = quantize_rows(weight)                       # [features, depth], once
     x = norm_quantize(y, gain, bias, residual=r, norm_out=r)
@@ -31,6 +32,7 @@ _grad_on = torch.is_grad_enabled
 _current_device = torch._C._cuda_getDevice            # (torch.cuda.current_device without its init check:
 _current_stream = torch._C._cuda_getCurrentRawStream  # the operands are device tensors; 0.1 us against 1.4)
 _new = object.__new__
+_wrote = torch._C._increment_version                  # (torch.autograd.graph.increment_version of several tensors)
 _pack_norm = NORM_QUANT_ARGS.pack
 
 
@@ -178,9 +180,11 @@ def quantize_rows(x: torch.Tensor, act: str = "none", out: Optional[Int8Rows] = 
     if act not in _ACT:
         raise ValueError(f"unknown activation {act!r} (none | gelu)")
     rows, cols = x.shape
-    out = _int8_out(out, rows, cols, x)
+    given, out = out, _int8_out(out, rows, cols, x)
     _quant(device, x.data_ptr(), _DTYPE[x.dtype], _ld(x), rows, cols, _ACT[act], out._q.data_ptr(), _ld(out._q),
            out._scale.data_ptr())
+    if given is not None:
+        _wrote((out._q, out._scale))
     return out
 
 
@@ -225,11 +229,17 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     if norm_out is not None:
         norm_t, norm_ld = _rows_operand(norm_out, "norm_out", shape, device)
         norm_p = norm_out.data_ptr()
-    out = _int8_out(out, rows, cols, x)
+    given, out = out, _int8_out(out, rows, cols, x)
     q = out._q
     _norm_quant(device, _pack_norm(x.data_ptr(), _ld(x), resid_p, resid_ld, weight.data_ptr(), bias_p, sum_p, sum_ld,
                                    norm_p, norm_ld, q.data_ptr(), _ld(q), out._scale.data_ptr(), rows, cols,
                                    _DTYPE[x.dtype], resid_t, norm_t, _NORM[norm], eps))
+    if given is not None:
+        _wrote((q, out._scale))
+    if sum_out is not None:
+        _wrote((sum_out,))
+    if norm_out is not None:
+        _wrote((norm_out,))
     return out
 
 
@@ -267,12 +277,15 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None,
         code = _DTYPE.get(dtype)
         if code is None:
             raise ValueError(f"dtype {dtype} is not supported here")
-        out = xq.new_empty((rows, features), dtype=dtype)
+        given, out = False, xq.new_empty((rows, features), dtype=dtype)
         ldo = features
     else:
+        given = True
         code, ldo = _rows_operand(out, "out", (rows, features), device)
     _linear(device, xq.data_ptr(), _ld(xq), x._scale.data_ptr(), rows, wq.data_ptr(), _ld(wq), w._scale.data_ptr(),
             features, depth, bias_p, out.data_ptr(), code, ldo)
+    if given:
+        _wrote((out,))
     return out
 
 

@@ -43,3 +43,53 @@ def test_restored_host_rows_are_refused():
         _host_rows(0, 32).dequantize()
     with pytest.raises(ValueError, match="device tensor"):
         m.quantize_rows(torch.zeros(4, 32), out=x)
+
+
+# ---- gradients: refused, never dropped in silence ---------------------------------------------
+def _norm_buffers():
+    x, r = torch.randn(5, 96, device="cuda"), torch.randn(5, 96, device="cuda")
+    return x, r, torch.ones(96, device="cuda")
+
+
+def _written(m):
+    """(name, the buffer, a call that writes it) for every buffer that a caller may hand out."""
+    x, r, g = _norm_buffers()
+    rows, w = m.quantize_rows(x), m.quantize_rows(torch.randn(7, 96, device="cuda"))
+    out, y = m.Int8Rows.empty(5, 96, x.device), torch.empty(5, 7, device="cuda")
+    total, normed = torch.empty_like(r), torch.empty_like(r)
+    yield "sum_out", total, lambda: m.norm_quantize(x, g, residual=r, sum_out=total)
+    yield "norm_out", normed, lambda: m.norm_quantize(x, g, residual=r, norm_out=normed)
+    yield "residual", r, lambda: m.norm_quantize(x, g, residual=r, norm_out=r)
+    yield "norm scale", out.scale, lambda: m.norm_quantize(x, g, out=out)
+    yield "norm q", out.q, lambda: m.norm_quantize(x, g, out=out)
+    yield "scale", out.scale, lambda: m.quantize_rows(x, out=out)
+    yield "q", out.q, lambda: m.quantize_rows(x, out=out)
+    yield "out", y, lambda: m.int8_linear(rows, w, out=y)
+
+
+@pytest.mark.gpu
+def test_writes_are_seen_by_autograd():
+    """A buffer that a backward pass has saved and an operator overwrites: the backward raises."""
+    for name, buf, call in _written(_ops()):
+        buf.zero_()
+        before = buf._version
+        call()
+        assert buf._version > before, name
+        if buf.is_floating_point():
+            a = torch.ones_like(buf, requires_grad=True)
+            (a * buf).sum().backward()                      # nothing written in between: fine
+            saved = (a * buf).sum()
+            call()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                saved.backward()
+
+
+@pytest.mark.gpu
+def test_writes_to_inference_tensors():
+    """They keep no version: written all the same, in the mode and (the call has no gradient) outside."""
+    m = _ops()
+    with torch.inference_mode():
+        x, r, g = _norm_buffers()
+        m.norm_quantize(x, g, residual=r, norm_out=r)
+    with torch.no_grad():
+        m.norm_quantize(x, g, residual=r, norm_out=r)
