@@ -98,11 +98,12 @@ def _device(t, name: str, dtypes, dim: int) -> int:
 
 
 def _rows_device(r: "Int8Rows", name: str) -> int:
-    """The device index of int8 rows, which a loader may have restored to the host."""
+    """The device index of int8 rows, which a loader may have restored to the host and whose scales may
+    ask for a gradient since they were wrapped."""
     device = r._q.get_device()
     if device < 0:
         _refuse(r._q, name, (_I8,), 2)
-    if r._scale.get_device() != device:
+    if r._scale.get_device() != device or r._scale.requires_grad and _grad_on():
         _refuse(r._scale, name + ".scale", (_F32,), 1, device)
     return device
 

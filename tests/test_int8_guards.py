@@ -93,3 +93,23 @@ def test_writes_to_inference_tensors():
         m.norm_quantize(x, g, residual=r, norm_out=r)
     with torch.no_grad():
         m.norm_quantize(x, g, residual=r, norm_out=r)
+
+
+@pytest.mark.gpu
+def test_scales_that_ask_for_a_gradient_are_refused():
+    m = _ops()
+    q = torch.ones(4, 32, dtype=torch.int8, device="cuda")
+    with torch.no_grad():
+        wrapped = m.Int8Rows(q, torch.ones(4, device="cuda", requires_grad=True))
+    later = m.Int8Rows(q, torch.ones(4, device="cuda"))
+    later.scale.requires_grad_()
+    plain = m.Int8Rows(q, torch.ones(4, device="cuda"))
+    for rows in (wrapped, later):
+        for call in (lambda: m.int8_linear(rows, plain), lambda: m.int8_linear(plain, rows), lambda: rows.dequantize(),
+                     lambda: m.quantize_rows(torch.ones(4, 32, device="cuda"), out=rows),
+                     lambda: m.norm_quantize(torch.ones(4, 32, device="cuda"), torch.ones(32, device="cuda"), out=rows)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        with torch.no_grad():
+            assert torch.equal(m.int8_linear(rows, plain), m.int8_linear(plain, plain))
+            assert bool((rows.dequantize() == 1).all())
