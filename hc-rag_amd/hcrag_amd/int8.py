@@ -8,7 +8,7 @@ rows) are the pieces that ``BertEncoder(dtype="i8")`` runs its layers on; they b
 
 Every call is enqueued on torch's current stream of the tensors' device and returns at once;
 calls can be captured into graphs.  They compute no gradients: a tensor that asks for one is
-refused while gradients are recorded, and what a call writes into (``out``, ``sum_out``, ``norm_out``)
+refused while gradients are recorded, a forward-mode dual tensor always, and what a call writes into (``out``, ``sum_out``, ``norm_out``)
 counts as modified in place.  No CPU fallback: without the HIP library they raise.
 
     w = quantize_rows(weight)                       # [features, depth], once
@@ -20,6 +20,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from ._lib import (HCR_ACT_GELU, HCR_ACT_NONE, HCR_BF16, HCR_F16, HCR_F32, HCR_NORM_LAYER,
                    HCR_NORM_RMS, NORM_QUANT_ARGS, check, lib)
@@ -36,13 +37,18 @@ _wrote = torch._C._increment_version                  # (torch.autograd.graph.in
 _pack_norm = NORM_QUANT_ARGS.pack
 
 
+def _tangent(t) -> bool:
+    """Whether t carries a forward-mode tangent."""
+    return _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None
+
+
 # A single token's call is bound by what the host does, so the checks are one expression per
 # operand, the error message is put together only when it fails, and the C functions are looked up
 # once.
 def _ok(t, dtypes, dim: int, device: int) -> bool:
     return (isinstance(t, _Tensor) and t.dtype in dtypes and t.dim() == dim and t.get_device() == device >= 0
             and (t.is_contiguous() or t.shape[-1] <= 1 or t.stride(-1) == 1)
-            and not (t.requires_grad and _grad_on()))
+            and not (t.requires_grad and _grad_on()) and (_forward._current_level < 0 or not _tangent(t)))
 
 
 class _Entry:
@@ -84,7 +90,7 @@ def _refuse(t, name: str, dtypes, dim: int, device: Optional[int] = None) -> Non
         raise ValueError(f"{name}: expected a device tensor")
     if device is not None and t.get_device() != device:
         raise ValueError(f"{name}: on {t.device}, other operands on cuda:{device}")
-    if t.requires_grad and _grad_on():
+    if t.requires_grad and _grad_on() or _tangent(t):
         raise ValueError(f"{name}: requires a gradient, which the int8 operators do not compute")
     raise ValueError(f"{name}: elements of a row must be contiguous")
 
@@ -103,8 +109,9 @@ def _rows_device(r: "Int8Rows", name: str) -> int:
     device = r._q.get_device()
     if device < 0:
         _refuse(r._q, name, (_I8,), 2)
-    if r._scale.get_device() != device or r._scale.requires_grad and _grad_on():
-        _refuse(r._scale, name + ".scale", (_F32,), 1, device)
+    scale = r._scale
+    if scale.get_device() != device or scale.requires_grad and _grad_on() or _forward._current_level >= 0 and _tangent(scale):
+        _refuse(scale, name + ".scale", (_F32,), 1, device)
     return device
 
 

@@ -113,3 +113,26 @@ def test_scales_that_ask_for_a_gradient_are_refused():
         with torch.no_grad():
             assert torch.equal(m.int8_linear(rows, plain), m.int8_linear(plain, plain))
             assert bool((rows.dequantize() == 1).all())
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    m = _ops()
+    x, r, g = _norm_buffers()
+    rows = m.quantize_rows(x)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))                  # noqa: E731
+        wrapped = object.__new__(m.Int8Rows)                                  # (past the constructor's own check)
+        wrapped._q, wrapped._scale = rows.q, dual(rows.scale)
+        for call in (lambda: m.quantize_rows(dual(x)), lambda: m.norm_quantize(dual(x), g),
+                     lambda: m.norm_quantize(x, dual(g)), lambda: m.norm_quantize(x, g, bias=dual(g)),
+                     lambda: m.norm_quantize(x, g, residual=dual(r)), lambda: m.Int8Rows(rows.q, dual(rows.scale)),
+                     lambda: m.int8_linear(rows, rows, bias=dual(g[:5].contiguous())), lambda: m.int8_linear(wrapped, rows),
+                     lambda: m.int8_linear(rows, wrapped), lambda: wrapped.dequantize(),
+                     lambda: m.quantize_rows(x, out=wrapped)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+                call()
+        assert torch.equal(m.quantize_rows(x).q, rows.q)                      # no tangent: as ever
