@@ -32,10 +32,11 @@ typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 // -------------------------------------------------------------------------------------
 
 // gelu(x) = x Phi(x) = x / (1 + 2^-z), z = log2(Phi / (1 - Phi)) = x g(x^2): g as a polynomial fitted so
-// that Phi is within 2.9e-8 everywhere (its last coefficient is positive: z keeps x's sign past the
+// that Phi is within 3.6e-8 everywhere (its last coefficient is positive: z keeps x's sign past the
 // fit, where Phi is 0 or 1).  Fewer instructions than erf_as's form, whose error in Phi it also halves:
-// this kernel is bound by arithmetic (65521 x 4096: 207 us with erf_as, 160 so).  In fp32
-// |dv| <= 0.4 (1.6e-7 |x| + 2.4e-7 |v|).
+// this kernel is bound by arithmetic (65521 x 4096: 207 us with erf_as, 160 so).  In fp32, exp2 and the
+// reciprocal each off by one ulp at most, |dv| <= 0.81 (1.6e-7 |x| + 2.4e-7 |v|).  That is an absolute
+// bound: in the negative tail nothing of v may be left (i8_gelu_tail).
 __device__ __forceinline__ float i8_gelu(float x) {
   const float t = x * x;
   float g = 5.067230635091846e-09f;
@@ -46,6 +47,26 @@ __device__ __forceinline__ float i8_gelu(float x) {
   g = fmaf(g, t, 1.0483512282371521e-01f);
   g = fmaf(g, t, 2.3022093772888184e+00f);
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-(g * x)));
+}
+
+// gelu(x) relative to itself, for the rows whose scale is a value of the negative tail: no element of such
+// a row is larger than I8_GELU_SMALL, so it is either below -3 (x Phi(x) = -phi(x) W(1 / x^2), W as a
+// polynomial fitted within 5e-7 for x < -2.5, phi the normal density with its factor in W's coefficients)
+// or within 0.008 of 0, where the logistic form is relative already.
+// |dv| <= (1e-6 + (1.25 x^2 + 24) 2^-24) |v|.  65521 x 4096 f16: rows in the tail 249 us, others 163
+// (without this branch 161), rows of zeros 144.
+constexpr uint32_t I8_GELU_SMALL = 0x3B800000u;        // 2^-8, as bits
+__device__ __forceinline__ float i8_gelu_tail(float x) {
+  const float t = x * x, s = __builtin_amdgcn_rcpf(t);
+  float p = 105.96810913085938f;
+  p = fmaf(p, s, -73.01840209960938f);
+  p = fmaf(p, s, 23.39447784423828f);
+  p = fmaf(p, s, -5.247370719909668f);
+  p = fmaf(p, s, 1.1810914278030396f);
+  p = fmaf(p, s, -0.39880889654159546f);
+  p = fmaf(p, s, 0.39894208312034607f);
+  const float tail = -(__builtin_amdgcn_exp2f(t * -0.72134752044448f) * p);   // (log2(e) / 2)
+  return x < -2.5f ? tail : i8_gelu(x);
 }
 
 // v inv, rounded, plus 1.5 * 2^23, rounded: the low byte is v inv to the nearest whole number, ties to
@@ -193,7 +214,7 @@ __device__ __forceinline__ float i8_row_sum(float s, uint32_t* red, int wave, in
 // vectors, each half of its lines, and the int8 rows of a mere quantisation: 65521 x 4096 f16 118 us, with
 // them 125).
 template <int MODE, int WAVES, int NCH, bool NT>
-__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 1 && MODE == I8_GELU ? 8 : 1)
 rows_to_int8_kernel(I8RowArgs a) {
   __shared__ uint32_t red[WAVES > 1 ? WAVES : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -313,19 +334,47 @@ rows_to_int8_kernel(I8RowArgs a) {
   }
   // the largest pattern as signed (of the positive elements) and as unsigned (of the negative ones,
   // if there are any): one three-way maximum per two elements each
-  int mp = 0;
-  uint32_t mn = 0u;
+  uint32_t mn;
+  auto largest = [&]() __attribute__((always_inline)) {
+    int mp = 0;
+    mn = 0u;
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+    for (int c = 0; c < NCH; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const uint32_t u0 = __float_as_uint(v[c][e]), u1 = __float_as_uint(v[c][e + 1]);
-      mp = max(max(mp, (int)u0), (int)u1);
-      mn = max(max(mn, u0), u1);
+      for (int e = 0; e < 8; e += 2) {
+        const uint32_t u0 = __float_as_uint(v[c][e]), u1 = __float_as_uint(v[c][e + 1]);
+        mp = max(max(mp, (int)u0), (int)u1);
+        mn = max(max(mn, u0), u1);
+      }
+    uint32_t m = max((uint32_t)mp, (mn >> 31) ? mn & 0x7FFFFFFFu : 0u);
+    if (overflow) m = 0x7FC00000u;
+    return i8_row_reduce<WAVES>(m, red, wave, lane, [](uint32_t p, uint32_t q) { return max(p, q); });
+  };
+  uint32_t m = largest();
+  if constexpr (MODE == I8_GELU) {
+    if ((uint32_t)__builtin_amdgcn_readfirstlane((int)m) < I8_GELU_SMALL) {
+      // (v keeps x's sign, also where nothing is left of it: rows of zeros, as padding is, end here)
+      const int negative = (int)(mn >> 31);
+      if (WAVES == 1 ? __any(negative) : __syncthreads_or(negative)) {
+        // The row again, relative to its values.  Read again, a chunk at a time: held for this, its
+        // elements would cost every row registers.  (The address is one that the compiler cannot take for
+        // the first reads'.)
+        const char* xa = xr;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+          const int i = (tid + NTH * c) * 8, n = a.cols - i;
+          asm volatile("" : "+v"(xa)::"memory");
+          I8Raw raw;
+          if (x32) i8_load<true>(raw, xa, i, a.cols);
+          else i8_load<false>(raw, xa, i, a.cols);
+          i8_convert(v[c], raw, a.xt);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[c][e] = e < n ? i8_gelu_tail(v[c][e]) : 0.f;
+        }
+        m = largest();
+      }
     }
-  uint32_t m = max((uint32_t)mp, (mn >> 31) ? mn & 0x7FFFFFFFu : 0u);
-  if (overflow) m = 0x7FC00000u;
-  m = i8_row_reduce<WAVES>(m, red, wave, lane, [](uint32_t p, uint32_t q) { return max(p, q); });
+  }
   const float amax = __uint_as_float(m);
   const bool bad = m >= 0x7F800000u;
   const bool zero = bad || amax < 0x1p-100f;

@@ -372,7 +372,8 @@ int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_m
  * ------------------------------------------------------------------------------------- */
 
 /* v = activation(x): int8 rows of x [rows][cols] (x_dtype HCR_F16 / HCR_BF16 / HCR_F32).  Weights
- * [features][depth] are laid out by the same call: a channel is a row. */
+ * [features][depth] are laid out by the same call: a channel is a row.  GELU is computed within
+ * 2^-21 |x|; in rows whose largest |v| is below 2^-8 (in the negative tail, say) within 1.3e-5 |v|. */
 int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols,
                           int activation, int8_t* d_q, int64_t ldq, float* d_scale, void* stream);
 
