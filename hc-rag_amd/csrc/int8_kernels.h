@@ -269,7 +269,6 @@ rows_to_int8_kernel(I8RowArgs a) {
       for (int e = 0; e < 8; ++e) v[c][e] = e < n ? v[c][e] : 0.f;
     }
   }
-  bool overflow = false;
   if constexpr (NORM) {
     float mean = 0.f;
     if constexpr (MODE == I8_LAYER) {
@@ -294,8 +293,8 @@ rows_to_int8_kernel(I8RowArgs a) {
       for (int e = 0; e < 8; ++e) s = fmaf(d[e], d[e], s);
     }
     const float var = i8_row_sum<WAVES>(s, red, wave, lane) / (float)a.cols;
-    overflow = !(var < INFINITY);  // the squares left fp32's range: the row is not representable
-    const float rstd = rsqrtf(var + a.eps);
+    // (squares past fp32's range: the row is not representable, and all of it becomes NaN)
+    const float rstd = var < INFINITY ? rsqrtf(var + a.eps) : __uint_as_float(0x7FC00000u);
     if (a.sum) {
       char* sr = reinterpret_cast<char*>(a.sum) + row * a.ldsum * (r32 ? 4 : 2);
 #pragma unroll
@@ -346,8 +345,7 @@ rows_to_int8_kernel(I8RowArgs a) {
         mp = max(max(mp, (int)u0), (int)u1);
         mn = max(max(mn, u0), u1);
       }
-    uint32_t m = max((uint32_t)mp, (mn >> 31) ? mn & 0x7FFFFFFFu : 0u);
-    if (overflow) m = 0x7FC00000u;
+    const uint32_t m = max((uint32_t)mp, (mn >> 31) ? mn & 0x7FFFFFFFu : 0u);
     return i8_row_reduce<WAVES>(m, red, wave, lane, [](uint32_t p, uint32_t q) { return max(p, q); });
   };
   uint32_t m = largest();

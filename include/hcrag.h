@@ -367,8 +367,8 @@ int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_m
  *
  * Quantisation of a row v: a = max |v|, scale = a / 127, q = round_half_even(v * (127 / a)), in
  * fp32.  a < 2^-100: the row counts as zeros (q 0, scale 0).  A row that holds a NaN or an
- * infinity, or whose squares leave fp32's range in a norm, gets q 0 and scale NaN, so that what is
- * computed from it is NaN.
+ * infinity, or whose squares leave fp32's range in a norm, gets q 0 and scale NaN (and a norm's
+ * output NaN), so that what is computed from it is NaN.
  * ------------------------------------------------------------------------------------- */
 
 /* v = activation(x): int8 rows of x [rows][cols] (x_dtype HCR_F16 / HCR_BF16 / HCR_F32).  Weights

@@ -1,5 +1,5 @@
 """Rows of the 8-bit integer operators where absolute bounds say nothing: GELU rows that lie wholly in the
-negative tail.
+negative tail, rows of a norm whose squares leave fp32's range.
 
 GELU, u = 2^-24, exp2 and the reciprocal within one ulp (2 u).  A row of amax >= 2^-8 is x Phi(x) with Phi
 from a fitted logistic form 1 / (1 + 2^w): the fit is within 3.6e-8 of Phi, w = -g(x^2) x is off by 4 u |w|
@@ -87,3 +87,31 @@ def test_gelu_rows_that_are_not_finite(cols):
     r = m.quantize_rows(x, act="gelu")
     assert bool(r.scale[:3].isnan().all()) and bool((r.q[:3] == 0).all())
     assert bool((r.q[3] == -127).all())
+
+
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("yt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("cols", [33, 900, 2500, 6000])
+def test_norm_output_of_rows_past_fp32_is_nan(cols, yt, norm):
+    """A row whose squares leave fp32's range: not only its scale but its normalised row is NaN, so that a
+    residual stream does not go on from the bias; its neighbours and the stored sum are as ever."""
+    m, g = _ops(), _gen(cols)
+    weight = 1 + 0.2 * torch.randn(cols, generator=g, device="cuda")
+    bias = 0.3 * torch.randn(cols, generator=g, device="cuda")
+    x = torch.randn(5, cols, generator=g, device="cuda")
+    r = torch.randn(5, cols, generator=g, device="cuda")
+    for b in (None, bias):
+        want_y = torch.empty(5, cols, device="cuda", dtype=DT[yt])
+        want = m.norm_quantize(x, weight, b, residual=r, norm=norm, eps=1e-6, norm_out=want_y)
+        big = x.clone()
+        big[1] *= 1e25
+        big[3] = 3e38 * torch.sign(x[3])
+        big[4, :] = 0.0
+        big[4, cols - 1] = 1e20
+        y, total = torch.zeros(5, cols, device="cuda", dtype=DT[yt]), torch.empty(5, cols, device="cuda")
+        out = m.norm_quantize(big, weight, b, residual=r, norm=norm, eps=1e-6, norm_out=y, sum_out=total)
+        assert bool(y[[1, 3, 4]].isnan().all())
+        assert bool(out.scale[[1, 3, 4]].isnan().all()) and bool((out.q[[1, 3, 4]] == 0).all())
+        assert torch.equal(total, big + r)
+        assert torch.equal(y[[0, 2]], want_y[[0, 2]])
+        assert torch.equal(out.q[[0, 2]], want.q[[0, 2]]) and torch.equal(out.scale[[0, 2]], want.scale[[0, 2]])
