@@ -145,9 +145,7 @@ class Int8Rows:
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Int8Rows":
         """Uninitialised rows on a GPU, laid out as the operators want them."""
-        self = _new(cls)
-        self._q = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=_I8, device=device)
-        self._scale = torch.empty(rows, dtype=_F32, device=device)
+        self = _empty_rows(cls, rows, cols, device)
         _rows_device(self, "rows")
         return self
 
@@ -173,9 +171,16 @@ class Int8Rows:
         return out
 
 
+def _empty_rows(cls, rows: int, cols: int, device) -> Int8Rows:
+    self = _new(cls)
+    self._q = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=_I8, device=device)
+    self._scale = torch.empty(rows, dtype=_F32, device=device)
+    return self
+
+
 def _int8_out(out: Optional[Int8Rows], rows: int, cols: int, like: torch.Tensor) -> Int8Rows:
     if out is None:
-        return Int8Rows.empty(rows, cols, like.device)
+        return _empty_rows(Int8Rows, rows, cols, like.device)
     if tuple(out._q.shape) != (rows, cols) or _rows_device(out, "out") != like.get_device():
         raise ValueError(f"out: {tuple(out._q.shape)} on {out._q.device}, expected {(rows, cols)} on {like.device}")
     return out
