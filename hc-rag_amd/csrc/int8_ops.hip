@@ -3,6 +3,8 @@
 // every call can be captured into a graph and run from several threads and streams at once.
 #include <hip/hip_runtime.h>
 
+#include <initializer_list>
+
 #include "int8_kernels.h"
 #include "int8_gemm.h"
 #include "int8_ops.h"
@@ -214,8 +216,11 @@ static int check_same(const char* what, const void* p, int dt, int64_t ld, const
     return hcr_set_errorf(HCR_EINVAL, "%s in the buffer of %s: needs its dtype and row stride", what, other);
   return HCR_OK;
 }
-static int check_apart(const char* what, const void* p, const char* other, const void* o) {
-  return p && p == o ? hcr_set_errorf(HCR_EINVAL, "%s and %s must not overlap", what, other) : HCR_OK;
+struct Operand { const char* what; const void* p; };
+static int check_apart(const Operand& out, std::initializer_list<Operand> others) {
+  for (const Operand& o : others)
+    if (out.p && out.p == o.p) return hcr_set_errorf(HCR_EINVAL, "%s and %s must not overlap", out.what, o.what);
+  return HCR_OK;
 }
 
 extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, int act,
@@ -227,7 +232,8 @@ extern "C" int hcr_quant_rows_device(const void* d_x, int x_dtype, int64_t ldx, 
   CHECK(check_floats("x", d_x, x_dtype, ldx, cols));
   CHECK(check_int8("q", d_q, ldq, cols));
   if (!on(d_scale, 4)) return hcr_set_error(HCR_EINVAL, "scale: not aligned to its elements");
-  CHECK(check_apart("q", d_q, "x", d_x));
+  CHECK(check_apart({"q", d_q}, {{"x", d_x}}));
+  CHECK(check_apart({"scale", d_scale}, {{"x", d_x}, {"q", d_q}}));
   I8RowArgs a{};
   a.x = d_x; a.ldx = ldx; a.xt = x_dtype;
   a.q = d_q; a.ldq = ldq; a.scale = d_scale; a.rows = rows; a.cols = (int)cols;
@@ -253,12 +259,12 @@ extern "C" int hcr_norm_quant_rows_device(const hcr_norm_quant_args* args, void*
   CHECK(check_same("the sum", n.sum, n.residual_dtype, n.ldsum, "the residual", n.residual, n.residual_dtype, n.ldr));
   CHECK(check_same("the norm output", n.norm_out, n.norm_dtype, n.ldnorm, "x", n.x, n.x_dtype, n.ldx));
   CHECK(check_same("the norm output", n.norm_out, n.norm_dtype, n.ldnorm, "the residual", n.residual, n.residual_dtype, n.ldr));
-  CHECK(check_apart("the sum", n.sum, "x", n.x));
-  CHECK(check_apart("the sum", n.sum, "the norm output", n.norm_out));
-  CHECK(check_apart("q", n.q, "x", n.x));
-  CHECK(check_apart("q", n.q, "the residual", n.residual));
-  CHECK(check_apart("q", n.q, "the sum", n.sum));
-  CHECK(check_apart("q", n.q, "the norm output", n.norm_out));
+  const Operand x{"x", n.x}, residual{"the residual", n.residual}, weight{"weight", n.weight}, bias{"bias", n.bias},
+      sum{"the sum", n.sum}, norm_out{"the norm output", n.norm_out}, q{"q", n.q};
+  CHECK(check_apart(sum, {x, weight, bias, norm_out}));
+  CHECK(check_apart(norm_out, {weight, bias}));
+  CHECK(check_apart(q, {x, residual, weight, bias, sum, norm_out}));
+  CHECK(check_apart({"scale", n.scale}, {x, residual, weight, bias, sum, norm_out, q}));
   I8RowArgs a{};
   a.x = n.x; a.ldx = n.ldx; a.xt = n.x_dtype;
   a.r = n.residual; a.ldr = n.ldr; a.rt = n.residual ? n.residual_dtype : HCR_F32;
@@ -277,7 +283,7 @@ extern "C" int hcr_dequant_rows_device(const int8_t* d_q, int64_t ldq, const flo
   CHECK(check_int8("q", d_q, ldq, cols));
   CHECK(check_floats("out", d_out, out_dtype, ldo, cols));
   if (!on(d_scale, 4)) return hcr_set_error(HCR_EINVAL, "scale: not aligned to its elements");
-  CHECK(check_apart("out", d_out, "q", d_q));
+  CHECK(check_apart({"out", d_out}, {{"q", d_q}, {"scale", d_scale}}));
   if (rows * cols > kI8MaxElements) return hcr_set_error(HCR_EINVAL, "more than 2^40 elements");
   const int64_t per = (cols + 7) / 8, most = kLaunchThreads / per;   // threads per row, rows per launch
   for (int64_t r = 0; r < rows; r += most) {
@@ -305,8 +311,7 @@ extern "C" int hcr_int8_linear_device(const int8_t* d_x, int64_t ldx, const floa
   CHECK(check_floats("out", d_out, out_dtype, ldo, features));
   if (!on(d_x_scale, 4) || !on(d_w_scale, 4) || !on(d_bias, 4))
     return hcr_set_error(HCR_EINVAL, "scales or bias: not aligned to their elements");
-  CHECK(check_apart("out", d_out, "x", d_x));
-  CHECK(check_apart("out", d_out, "w", d_w));
+  CHECK(check_apart({"out", d_out}, {{"x", d_x}, {"w", d_w}, {"x's scale", d_x_scale}, {"w's scale", d_w_scale}, {"bias", d_bias}}));
   if (rows * features > kI8MaxElements) return hcr_set_error(HCR_EINVAL, "more than 2^40 outputs");
   I8LinearArgs a{};
   a.x = d_x; a.ldx = ldx; a.sx = d_x_scale;

@@ -45,6 +45,42 @@ def test_restored_host_rows_are_refused():
         m.quantize_rows(torch.zeros(4, 32), out=x)
 
 
+# ---- outputs in the place of vectors, scales in the place of anything: refused before any HIP call ----
+def _distinct():
+    """Arguments of the four C entry points, every buffer in a place of its own (never read: what is
+    called here is refused)."""
+    from hcrag_amd import _lib
+    lib = _lib.lib()
+    places = {n: (i + 1) << 24 for i, n in enumerate("x r w b s y q scale out sx sw".split())}
+
+    def quant(x, q, scale, **_):
+        return lib.hcr_quant_rows_device(x, _lib.HCR_F32, 64, 4, 64, 0, q, 64, scale, None)
+
+    def norm(x, r, w, b, s, y, q, scale, **_):
+        return lib.hcr_norm_quant_rows_device(_lib.NORM_QUANT_ARGS.pack(
+            x, 64, r, 64, w, b, s, 64, y, 64, q, 64, scale, 4, 64, _lib.HCR_F32, _lib.HCR_F32, _lib.HCR_F32, 0, 1e-6), None)
+
+    def dequant(q, scale, out, **_):
+        return lib.hcr_dequant_rows_device(q, 64, scale, 4, 64, out, _lib.HCR_F32, 64, None)
+
+    def linear(x, sx, w, sw, b, out, **_):
+        return lib.hcr_int8_linear_device(x, 64, sx, 4, w, 64, sw, 64, 64, b, out, _lib.HCR_F32, 64, None)
+
+    return places, dict(quant=quant, norm=norm, dequant=dequant, linear=linear)
+
+
+@pytest.mark.parametrize("call,output,operands", [
+    ("quant", "q", "x"), ("quant", "scale", "x q"),
+    ("norm", "scale", "x r w b s y q"), ("norm", "q", "x r w b s y"), ("norm", "s", "x w b y"), ("norm", "y", "w b"),
+    ("dequant", "out", "q scale"), ("linear", "out", "x sx w sw b")])
+def test_outputs_that_start_where_an_operand_does(call, output, operands):
+    from hcrag_amd import _lib
+    places, calls = _distinct()
+    for other in operands.split():
+        assert calls[call](**{**places, output: places[other]}) == _lib.HCR_EINVAL, other
+        assert b"overlap" in _lib.lib().hcr_last_error(), other
+
+
 # ---- gradients: refused, never dropped in silence ---------------------------------------------
 def _norm_buffers():
     x, r = torch.randn(5, 96, device="cuda"), torch.randn(5, 96, device="cuda")
