@@ -155,8 +155,10 @@ int int8_linear_launch(const I8LinearArgs& a, hipStream_t st) {
   const int64_t tmost = INT32_MAX / std::max<int64_t>(a.ldx, a.ldo * i8_size(a.ot)) / 256 * 256;
   const bool near = fmost > 0 && tmost > 0;
   const int64_t fstep = std::min<int64_t>(near ? fmost : a.N, 1 << 22);
-  // (far: the direct kernel's offsets have 64 bits; at most max(2^30, 512 * 2^22) threads a launch)
-  const int64_t tstep = near ? tmost : std::max<int64_t>((1 << 30) / std::min<int64_t>(a.N, fstep) / 64 * 64, 512);
+  // (far: the direct kernel's offsets have 64 bits; its workgroups take 32 features at most and a thread 4
+  // outputs, so 2^30 tokens x features, in whole 32s of features, are 2^28 threads, and 512 tokens 2^29)
+  const int64_t fwide = (std::min<int64_t>(a.N, fstep) + 31) / 32 * 32;
+  const int64_t tstep = near ? tmost : std::max<int64_t>((1 << 30) / fwide / 64 * 64, 512);
   for (int64_t f = 0; f < a.N; f += fstep) {
     I8LinearArgs c = a;
     c.N = (int)std::min(fstep, a.N - f);

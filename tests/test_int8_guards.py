@@ -172,3 +172,24 @@ def test_forward_mode_tangents_are_refused():
             with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
                 call()
         assert torch.equal(m.quantize_rows(x).q, rows.q)                      # no tangent: as ever
+
+
+# ---- launches ---------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_linear_far_rows_few_features():
+    """Weight rows 8 MiB apart and so many tokens that a launch over all of them would have 2^32 threads
+    (a workgroup takes 32 features, however few there are)."""
+    m = _ops()
+    T, N, K, ld = 2 ** 29, 2, 16, 2 ** 23 + 16
+    w = torch.zeros(N * ld, device="cuda", dtype=torch.int8).as_strided((N, K), (ld, 1))
+    w[0, 0], w[1, 1] = 2, -3
+    x = torch.zeros(T, K, device="cuda", dtype=torch.int8)
+    step = 2 ** 26
+    for t in range(0, T, step):
+        at = torch.arange(t, t + step, device="cuda")
+        x[t:t + step, 0], x[t:t + step, 1] = (at % 251 - 125).to(torch.int8), (at % 113 - 56).to(torch.int8)
+    y = m.int8_linear(m.Int8Rows(x, torch.ones(T, device="cuda")), m.Int8Rows(w, torch.ones(N, device="cuda")))
+    for t in range(0, T, step):
+        at = torch.arange(t, t + step, device="cuda")
+        assert torch.equal(y[t:t + step, 0], ((at % 251 - 125) * 2).to(y.dtype))       # (whole numbers that f16 holds)
+        assert torch.equal(y[t:t + step, 1], ((at % 113 - 56) * -3).to(y.dtype))
