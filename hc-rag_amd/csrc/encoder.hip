@@ -843,10 +843,12 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
   // (the last call may have used the first sub-batch's buffers on another stream)
   if (!e->work[0].done) HIPC(hipEventCreateWithFlags(&e->work[0].done, hipEventDisableTiming));
   HIPC(hipStreamWaitEvent(st, e->work[0].done, 0));
+  // A sub-batch that fails may have enqueued kernels (a sequence length past the attention's LDS shows
+  // after the first product): `done` is recorded, and the caller's stream waits, either way.
   if (splits == 1) {
-    CHECK(run(e->work[0], 0, n, st));
+    const int rc = run(e->work[0], 0, n, st);
     HIPC(hipEventRecord(e->work[0].done, st));
-    return HCR_OK;
+    return rc;
   }
   // Sub-batches of n / splits sequences, the first on the caller's stream, the others on streams of
   // their own (ordered after the caller's work through ev_in; the caller's stream waits for their
@@ -860,17 +862,19 @@ extern "C" int hcr_encode_device(hcr_encoder* e, const int32_t* d_ids, const int
     EncWork& w = e->work[i];
     const int64_t s0 = n * i / splits, s1 = n * (i + 1) / splits;
     if (i == 0) {
-      CHECK(run(w, s0, s1 - s0, st));
+      const int rc = run(w, s0, s1 - s0, st);
       HIPC(hipEventRecord(w.done, st));
+      CHECK(rc);
       continue;
     }
     // default priority: work on streams of different priorities has hung MI355X boards
     if (!w.st) HIPC(hipStreamCreateWithFlags(&w.st, hipStreamNonBlocking));
     if (!w.done) HIPC(hipEventCreateWithFlags(&w.done, hipEventDisableTiming));
     HIPC(hipStreamWaitEvent(w.st, e->ev_in, 0));
-    CHECK(run(w, s0, s1 - s0, w.st));
+    const int rc = run(w, s0, s1 - s0, w.st);
     HIPC(hipEventRecord(w.done, w.st));
     HIPC(hipStreamWaitEvent(st, w.done, 0));
+    CHECK(rc);
   }
   return HCR_OK;
 }

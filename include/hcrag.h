@@ -342,8 +342,9 @@ int hcr_encode(hcr_encoder* enc, const int32_t* ids, const int32_t* mask, int64_
  * run through the layers: the packed token count is read back once per call, so the call waits
  * for the caller's earlier work on `stream` and for the packing kernel; the layers are then
  * enqueued asynchronously (batches of >= 128 sequences -- HCR_I8: of more than 16384 positions too --
- * split over `stream` and an internal stream that `stream` waits for).  A call waits on the device
- * for the handle's last call, so calls one after the other may come on different streams. */
+ * split over `stream` and an internal stream that `stream` waits for).  A call waits for the
+ * handle's last call, also one that failed, so calls one after the other may come on different
+ * streams: the packing kernel waits on the device, and the host for it. */
 int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_mask, int64_t n,
                       int S, float* d_out, void* stream);
 
