@@ -15,7 +15,8 @@ from .ingest import BatchedEmbeddingGenerator, EmbeddingStore
 from . import relevance
 from . import graph_relevance
 
-# the int8 operators work on torch tensors: torch is imported when one of them is first asked for
+# the int8 operators work on torch tensors: torch is imported when one of them is first asked for by name
+# (`from hcrag_amd import *` leaves them out: it has to work, and fast, without torch)
 _INT8 = ("Int8Rows", "quantize_rows", "norm_quantize", "int8_linear")
 
 
@@ -28,10 +29,14 @@ def __getattr__(name):
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
+def __dir__():
+    return sorted({*globals(), *_INT8, "int8"})
+
+
 __version__ = "0.3.0"
 
 __all__ = ["VectorIndex", "MultiDeviceIndex", "merge_topk_device", "EmbeddingSearch", "batch_semantic_similarity",
            "WordPieceTokenizer", "BertEncoder", "SentenceEmbedder", "MI355XEmbedding", "config_from_hf",
            "MINILM_L6_V2", "device_count", "lib", "HcrError", "HCR_F16", "HCR_BF16", "HCR_F32",
            "HCR_SCORE_COSINE", "HCR_SCORE_UNIT", "BatchedEmbeddingGenerator", "EmbeddingStore",
-           "relevance", "graph_relevance", *_INT8]
+           "relevance", "graph_relevance"]

@@ -1,6 +1,9 @@
 """What the 8-bit integer operators refuse, or have to say, beyond their arguments' shapes: rows on the
 host, gradients and tensors that others have saved, buffers in each other's place."""
+import os
 import pickle
+import subprocess
+import sys
 
 import pytest
 
@@ -79,6 +82,17 @@ def test_outputs_that_start_where_an_operand_does(call, output, operands):
     for other in operands.split():
         assert calls[call](**{**places, output: places[other]}) == _lib.HCR_EINVAL, other
         assert b"overlap" in _lib.lib().hcr_last_error(), other
+
+
+# ---- the package without torch ----------------------------------------------------------------
+def test_star_import_does_not_need_torch():
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hc-rag_amd")
+    code = (f"import sys; sys.path.insert(0, {path!r}); sys.modules['torch'] = None\n"
+            "from hcrag_amd import *\n"
+            "import hcrag_amd; assert VectorIndex is hcrag_amd.VectorIndex and 'int8_linear' in dir(hcrag_amd)")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+    from hcrag_amd import Int8Rows, int8, int8_linear, norm_quantize, quantize_rows  # noqa: F401
 
 
 # ---- gradients: refused, never dropped in silence ---------------------------------------------
