@@ -19,6 +19,8 @@ D = torch.float64
 CONFIGS = {
     "heads of 64": dict(vocab_size=211, hidden=128, layers=2, heads=2, intermediate=256, max_position=160, type_vocab=2),
     "heads of 32": dict(vocab_size=97, hidden=192, layers=1, heads=6, intermediate=320, max_position=64, type_vocab=2),
+    "heads of 16": dict(vocab_size=97, hidden=64, layers=2, heads=4, intermediate=192, max_position=64, type_vocab=1),
+    "1088 wide": dict(vocab_size=97, hidden=1088, layers=1, heads=17, intermediate=2176, max_position=64, type_vocab=2),
 }
 LENS = [1, 2, 37, 36, 5, 17, 33, 3, 9, 10, 11, 12, 37]
 
