@@ -26,9 +26,10 @@ typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 // The maximum is taken over the bit patterns of |v|: an infinity or a NaN is larger than every
 // finite value, and such a row gets scale NaN and q = 0, so that a product with it is NaN.  A row
 // below 2^-100 counts as zeros (scale 0, q 0): 127 / a would leave fp32's range.
-// Bound by memory (MI355X; a copy of 8 GiB moves 4.6 TB/s): RMS norm with residual of 65521 x 4096 bf16
-// 1.88 GB in 345 us (5.4 TB/s), LayerNorm of 32749 x 768 (f16 + f32 -> f32) 52 us (5.3 TB/s), quantisation
-// of 65521 x 4096 f16 118 us (6.8 TB/s), with GELU 158 us, where arithmetic and memory meet.
+// Bound by memory (MI355X, calls back to back on one input; a copy of 8 GiB moves 4.6 TB/s): RMS norm with
+// residual of 65521 x 4096 bf16 1.88 GB in 317 us (5.9 TB/s), LayerNorm of 32749 x 768 (f16 + f32 -> f32)
+// 51 us (5.4 TB/s), quantisation of 65521 x 4096 f16 116 us (7.0 TB/s), with GELU 155-163 us by the board,
+// where arithmetic and memory meet.
 // -------------------------------------------------------------------------------------
 
 // gelu(x) = x Phi(x) = x / (1 + 2^-z), z = log2(Phi / (1 - Phi)) = x g(x^2): g as a polynomial fitted so
@@ -212,7 +213,7 @@ __device__ __forceinline__ float i8_row_sum(float s, uint32_t* red, int wave, in
 // One row per WAVES waves; WAVES == 1 puts 4 rows in a workgroup.  Covers cols <= 512 WAVES NCH.
 // NT: x, the residual and what is stored pass by the caches (but f32 rows, of which a lane takes two
 // vectors, each half of its lines, and the int8 rows of a mere quantisation: 65521 x 4096 f16 118 us, with
-// them 125).
+// them 125 on the same board).
 template <int MODE, int WAVES, int NCH, bool NT>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 1 && MODE == I8_GELU ? 8 : 1)
 rows_to_int8_kernel(I8RowArgs a) {

@@ -15,9 +15,9 @@ using namespace hcr;
 namespace hcr {
 
 // What a call reads or writes beyond the 256 MiB of the memory-side cache is evicted before its next
-// use, so it goes past the caches (quantisation of 65521 x 4096 f16 138 us, so 118; dequantisation
-// 139, 118; RMS norm 360, 345).  Below that the next kernel pays more than this one gains: 65521 x 768
-// f16, dequantisation and an addition 70 us, 77 so; quantisation and a product 70, 76.
+// use, so it goes past the caches (quantisation of 65521 x 4096 f16 137 us, so 116; dequantisation
+// 138, 116; RMS norm 328, 317; with GELU 160, 156).  Below that the next kernel pays more than this
+// one gains: 65521 x 768 f16, dequantisation and an addition 70 us, 77 so; quantisation and a product 70, 76.
 constexpr int64_t kNtBytes = (int64_t)256 << 20;
 
 constexpr int64_t kLaunchThreads = (int64_t)1 << 31;   // per launch; a grid of 2^32 threads is refused
@@ -85,7 +85,7 @@ static void launch_tile(const I8LinearArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((int8_linear_tiles<OT, ODD, MT, WM, WN, NST, OCC, NT>), dim3((unsigned)tiles_of(a, FT, TT)),
                      dim3(64 * WM * WN), 0, st, a, (a.N + FT - 1) / FT);
 }
-// Results of kNtBytes and more (T = 65536, K = 1024, N = 4096, f16, 512 MiB: 321 us, so 292; T = 24576, 192 MiB:
+// Results of kNtBytes and more (T = 65536, K = 1024, N = 4096, f16, 512 MiB: 319 us, so 297; T = 24576, 192 MiB:
 // 112, 115), unless rows are no whole number of 16 bytes (T = 30001, K = 777, N = 2051, f32: 127, 268).
 static bool nt_out(const I8LinearArgs& a) { return (int64_t)a.T * a.N * i8_size(a.ot) >= kNtBytes; }
 

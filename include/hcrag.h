@@ -356,8 +356,7 @@ int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_m
  * int8 rows: q [rows][cols] of int8 with one fp32 scale per row; element = q * scale.  q's rows
  * start on 16 bytes (16-byte aligned pointer, row stride ldq a multiple of 16; for one row too);
  * bytes of a row past its columns are neither read as values nor written.  Strides (ld*) are in
- * elements and at least the row's columns; other buffers need only their elements' alignment
- * (rows that start on 16 bytes are read and written in vectors).
+ * elements and at least the row's columns; other buffers need only their elements' alignment.
  *
  * Asynchronous on `stream` (a hipStream_t of the current device; NULL = the legacy default
  * stream).  Nothing is allocated, waited for or kept between calls: calls may run at once from
@@ -368,8 +367,8 @@ int hcr_encode_device(hcr_encoder* enc, const int32_t* d_ids, const int32_t* d_m
  *
  * Quantisation of a row v: a = max |v|, scale = a / 127, q = round_half_even(v * (127 / a)), in
  * fp32.  a < 2^-100: the row counts as zeros (q 0, scale 0).  A row that holds a NaN or an
- * infinity, or whose squares leave fp32's range in a norm, gets q 0 and scale NaN (and a norm's
- * output NaN), so that what is computed from it is NaN.
+ * infinity gets q 0 and scale NaN, so that what is computed from it is NaN; so does a row whose
+ * squares leave fp32's range in a norm, and its normalised elements are all NaN.
  * ------------------------------------------------------------------------------------- */
 
 /* v = activation(x): int8 rows of x [rows][cols] (x_dtype HCR_F16 / HCR_BF16 / HCR_F32).  Weights

@@ -4,8 +4,8 @@ by hcrag_amd.int8) against their definitions in 64 bits.
 Tolerances are bounds, from u = 2^-24 (half a step of fp32) and h = half a step of the output type:
   linear   float(acc), * sx, and the final fma round once each: 2.01 u |acc sx sw| + u |y| + h |y|
   quantise without an activation: q and scale are single IEEE fp32 operations, so bits are equal
-  gelu     erf within 3e-7 (Abramowitz & Stegun 7.1.26 plus the rcp / exp2 approximations) and four
-           roundings: |dv| <= 1.6e-7 |x| + 4 u |v|
+  gelu     Phi from a fitted logistic form (within 3.6e-8) plus the rcp / exp2 approximations and
+           four roundings, derived in test_int8_rows_gpu.py: |dv| <= 1.6e-7 |x| + 4 u |v|
   norm     _norm_bound below
   q of any v with error dv: |q - 127 v / a| <= 1/2 + 127 (dv + da) / a + 127 * 4 u, a = max |v|
 """
