@@ -8,8 +8,9 @@ rows) are the pieces that ``BertEncoder(dtype="i8")`` runs its layers on; they b
 
 Every call is enqueued on torch's current stream of the tensors' device and returns at once;
 calls can be captured into graphs.  They compute no gradients: a tensor that asks for one is
-refused while gradients are recorded, a forward-mode dual tensor always, and what a call writes into (``out``, ``sum_out``, ``norm_out``)
-counts as modified in place.  No CPU fallback: without the HIP library they raise.
+refused while gradients are recorded, a forward-mode dual tensor always, and what a call writes
+into (``out``, ``sum_out``, ``norm_out``) counts as modified in place.  No CPU fallback: without the
+HIP library they raise.
 
     w = quantize_rows(weight)                       # [features, depth], once
     x = norm_quantize(y, gain, bias, residual=r, norm_out=r)
